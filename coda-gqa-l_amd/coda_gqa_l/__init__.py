@@ -8,6 +8,7 @@ kernels of libcoda_mi355x.so (C ABI: include/coda_mi355x.h).
 from .adapters import EveCoDAAdapter, LlamaCoDAAdapter, Qwen3CoDAAdapter
 from .attention import CoDAGQALandmarkPerf2
 from .baseline import CoDAGQA
+from .int8 import Int8Rows, linear_int8, quantize_rows, rms_norm_int8
 from .memory_banks import MemoryBankMixin
 from .ops import diff_epilogue, diff_flash_attn, diff_sub_only, is_available
 from .primitives import HeadwiseRMSNorm, RotaryEmbedding, apply_rope, compute_lf_start, repeat_kv
@@ -29,5 +30,9 @@ __all__ = [
     "diff_flash_attn",
     "diff_epilogue",
     "diff_sub_only",
+    "Int8Rows",
+    "quantize_rows",
+    "rms_norm_int8",
+    "linear_int8",
     "is_available",
 ]

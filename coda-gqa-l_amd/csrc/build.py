@@ -23,7 +23,7 @@ from _srchash import source_hash  # noqa: E402  (no torch import)
 sys.path.pop(0)
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(PKG, "libcoda_mi355x.so")
-SOURCES = ["abi.hip", "attn.hip", "epilogue.hip", "rope.hip", "banks.hip", "proj.hip"]
+SOURCES = ["abi.hip", "attn.hip", "epilogue.hip", "rope.hip", "banks.hip", "proj.hip", "int8.hip"]
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
          # packed fp32 instructions are kept out of every kernel

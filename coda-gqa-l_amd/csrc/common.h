@@ -67,6 +67,10 @@ inline int device_cus() {
 
 // ----------------------------------------------------------------- types
 typedef uint16_t bf16_t;  // raw bfloat16 bits
+// half storage: a type of its own, so that traits tell it from bf16_t
+struct f16_t {
+  uint16_t v;
+};
 
 __host__ __device__ __forceinline__ float bf2f(bf16_t h) {
   return __builtin_bit_cast(float, (uint32_t)h << 16);
@@ -99,6 +103,13 @@ template <> struct Elt<bf16_t> {
   static __host__ __device__ __forceinline__ float ld(bf16_t x) { return bf2f(x); }
   static __host__ __device__ __forceinline__ bf16_t st(float x) { return f2bf(x); }
   static __host__ __device__ __forceinline__ float rnd(float x) { return bf2f(f2bf(x)); }
+};
+template <> struct Elt<f16_t> {
+  static __host__ __device__ __forceinline__ float ld(f16_t x) { return (float)__builtin_bit_cast(_Float16, x.v); }
+  static __host__ __device__ __forceinline__ f16_t st(float x) {
+    return f16_t{__builtin_bit_cast(uint16_t, (_Float16)x)};
+  }
+  static __host__ __device__ __forceinline__ float rnd(float x) { return ld(st(x)); }
 };
 
 // RoPE of one pair with (c, s), one rounding to T per multiply and add, as

@@ -6,23 +6,7 @@
 // :95-96): one rounding to the element type after every torch op.
 #include "common.h"
 
-#include <hip/hip_fp16.h>
-
 namespace coda {
-
-// half storage: a distinct type so the traits do not collide with bf16_t
-struct f16_t {
-  uint16_t v;
-};
-
-template <typename T> struct EpiElt;
-template <> struct EpiElt<float> : Elt<float> {};
-template <> struct EpiElt<bf16_t> : Elt<bf16_t> {};
-template <> struct EpiElt<f16_t> {
-  static __device__ __forceinline__ float ld(f16_t x) { return __half2float(__ushort_as_half(x.v)); }
-  static __device__ __forceinline__ f16_t st(float x) { return f16_t{__half_as_ushort(__float2half_rn(x))}; }
-  static __device__ __forceinline__ float rnd(float x) { return ld(st(x)); }
-};
 
 template <typename T, bool NORM>
 __global__ __launch_bounds__(256) void diff_epilogue_kernel(T* __restrict__ out, const T* __restrict__ sig,
@@ -30,7 +14,7 @@ __global__ __launch_bounds__(256) void diff_epilogue_kernel(T* __restrict__ out,
                                                             const T* __restrict__ lam,
                                                             const T* __restrict__ w, int rows, int dh,
                                                             float eps) {
-  using E = EpiElt<T>;
+  using E = Elt<T>;
   const int lane = threadIdx.x & 63;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;

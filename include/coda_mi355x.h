@@ -186,6 +186,48 @@ int coda_rows_pack(int dtype, const void* w, int n_feat, int D, int64_t w_sm, vo
  * keep their partial sums in LDS; kept for callers that size one). */
 int coda_project_workspace_bytes(const coda_proj_desc* d, size_t* bytes);
 
+/* ------------------------------------------------------------------------
+ * Rows in 8 bits: int8 codes in [-127, 127], one float scale a row, the
+ * value of a code being code * scale.  A row's codes lie at a 16-byte
+ * address and are followed by zeros up to a multiple of 128 bytes (row
+ * strides c_sm, x_sm, w_sm in bytes).  No counterpart in the reference,
+ * whose projections are float linears (src/coda_gqa_l/attention.py:396-410).
+ * dtype: CODA_F32, CODA_BF16 or CODA_F16; row strides of x, residual, out in
+ * elements; rows of at most 32768 elements.
+ * ---------------------------------------------------------------------- */
+
+/* Rows x (rows, D): scale = max|x| / 127, code = x / scale to the nearest,
+ * ties to even.  A row with an infinity or a NaN: scale NaN, codes 0; a row
+ * of zeros: scale 0.  Writes the zeros behind D too. */
+int coda_quantize_rows(int dtype, const void* x, int64_t x_sm, int rows, int D, int8_t* codes, int64_t c_sm,
+                       float* scales, void* stream);
+
+/* The same of y = s weight / sqrt(mean(s^2) + eps), s = x or, with a
+ * residual (may be NULL), x + residual rounded to dtype and written to
+ * sum_out (which may be x or residual itself). */
+int coda_rms_norm_int8(int dtype, const void* x, int64_t x_sm, const void* residual, int64_t r_sm, const void* weight,
+                       int rows, int D, float eps, void* sum_out, int64_t s_sm, int8_t* codes, int64_t c_sm,
+                       float* scales, void* stream);
+
+/* out (rows, D) = code * scale, one rounding to dtype. */
+int coda_dequantize_rows(int dtype, const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, void* out,
+                         int64_t o_sm, void* stream);
+
+/* out[m, f] = (sum_k x[m, k] w[f, k]) x_scales[m] w_scales[f] + bias[f], the
+ * sum exact in int32, one rounding to dtype.  K: the padded length, a
+ * multiple of 128 and at most 130944; bias (n_feat) of dtype, or NULL. */
+int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const float* x_scales, int M, const int8_t* w,
+                     int64_t w_sm, const float* w_scales, int n_feat, int K, const void* bias, void* out, int64_t o_sm,
+                     void* stream);
+
+/* The projection front end (coda_project) on rows in 8 bits, for any number
+ * of token rows: d->x (M, K) and d->w (n_feat, K) are codes (d->x_sm and w_sm
+ * in bytes, w row-major in coda_project's row order; D and w_layout unused),
+ * dtype CODA_BF16 or CODA_F32 the type of q, k, v, lam and the tables.
+ * gate == 0 leaves g alone (it may be NULL). */
+int coda_project_int8(const coda_proj_desc* d, const float* x_scales, const float* w_scales, int64_t w_sm, int K,
+                      void* stream);
+
 
 
 /* ------------------------------------------------------------------------

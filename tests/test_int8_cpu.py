@@ -1,0 +1,110 @@
+"""Rows in 8 bits: what is refused before any GPU call, and their layout."""
+import pytest
+import torch
+
+import coda_gqa_l
+from coda_gqa_l import Int8Rows, _hip
+
+
+def test_layout_of_rows():
+    c, s = torch.ones(2, 3, 100, dtype=torch.int8), torch.ones(2, 3)
+    r = Int8Rows.from_codes(c, s, torch.bfloat16)
+    assert r.codes.shape == (2, 3, 128) and r.shape == (2, 3, 100) and r.cols == 100 and not r.codes[..., 100:].any()
+    assert Int8Rows.from_codes(torch.ones(4, 256, dtype=torch.int8), torch.ones(4), torch.float32).codes.shape == (4, 256)
+
+
+@pytest.mark.parametrize("codes,scales,cols,dtype,error", [
+    (torch.zeros(2, 100, dtype=torch.int8), torch.zeros(2), 100, torch.float32, "last size must be 128"),
+    (torch.zeros(2, 256, dtype=torch.int8), torch.zeros(2), 100, torch.float32, "last size must be 128"),
+    (torch.zeros(2, 128, dtype=torch.int8), torch.zeros(3), 128, torch.float32, "scales"),
+    (torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2, 1), 128, torch.float32, "scales"),
+    (torch.zeros(2, 128, dtype=torch.uint8), torch.zeros(2), 128, torch.float32, "int8"),
+    (torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2).double(), 128, torch.float32, "int8"),
+    (torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), 0, torch.float32, "last size"),
+    (torch.zeros(2, 0, dtype=torch.int8), torch.zeros(2), 0, torch.float32, "last size"),
+])
+def test_rows_refused(codes, scales, cols, dtype, error):
+    with pytest.raises(RuntimeError, match=error):
+        Int8Rows(codes, scales, cols, dtype)
+
+
+def test_other_types_refused():
+    with pytest.raises(TypeError, match="dtype"):
+        Int8Rows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), 128, torch.int32)
+
+
+def test_no_host_path():
+    x = torch.zeros(2, 128)
+    r = Int8Rows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), 128, torch.float32)
+    for call in (lambda: coda_gqa_l.quantize_rows(x), lambda: coda_gqa_l.rms_norm_int8(x, x[0]),
+                 lambda: coda_gqa_l.linear_int8(r, r), r.dequantize):
+        with pytest.raises(RuntimeError, match="HIP devices only"):
+            call()
+
+
+P = 4096  # an address that no refused call reads
+
+
+@pytest.mark.parametrize("args,error", [
+    ((9, P, 64, 4, 64, P, 128, P), "dtype"),
+    ((1, P, 64, -1, 64, P, 128, P), "sizes"),
+    ((1, P, 64, 4, 0, P, 128, P), "sizes"),
+    ((1, P, 64, 4, 64, P, 64, P), "hold D=64"),
+    ((1, P, 64, 4, 64, P + 4, 128, P), "16-byte"),
+    ((1, P, 64, 4, 64, P, 136, P), "16-byte"),
+    ((1, P, 64, 4, 64, None, 128, P), "null"),
+    ((1, None, 64, 4, 64, P, 128, P), "null"),
+    ((1, P, 64, 4, 64, P, 128, None), "null"),
+])
+def test_quantize_rows_entry(args, error):
+    L = _hip.lib()
+    assert L.coda_quantize_rows(*args, None) == 1
+    assert error in L.coda_last_error().decode()
+
+
+def test_too_long_a_row_is_not_built():
+    L = _hip.lib()
+    assert L.coda_quantize_rows(1, P, 40000, 1, 40000, P, 40064, P, None) == _hip.CODA_EUNSUP
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(weight=None), "null"), (dict(sum_out=None), "null"), (dict(eps=-1.0), "negative"),
+    (dict(eps=float("nan")), "negative"), (dict(dtype=5), "dtype"),
+])
+def test_rms_norm_entry(change, error):
+    a = dict(dtype=1, x=P, x_sm=64, residual=P, r_sm=64, weight=P, rows=2, D=64, eps=1e-6, sum_out=P, s_sm=64, codes=P,
+             c_sm=128, scales=P)
+    a.update(change)
+    L = _hip.lib()
+    assert L.coda_rms_norm_int8(*a.values(), None) == 1
+    assert error in L.coda_last_error().decode()
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(K=64), "multiple of 128"), (dict(K=131072), "int32"), (dict(K=0), "sizes"), (dict(n_feat=0), "sizes"),
+    (dict(M=-1), "sizes"), (dict(x=P + 1), "16-byte"), (dict(w_sm=130), "16-byte"), (dict(w=None), "null"),
+    (dict(x=None), "null"), (dict(out=None), "output"), (dict(o_sm=9), "output"), (dict(dtype=3), "dtype"),
+    (dict(x_sm=-128), "16-byte"),
+])
+def test_linear_entry(change, error):
+    a = dict(dtype=1, x=P, x_sm=128, x_scales=P, M=3, w=P, w_sm=128, w_scales=P, n_feat=10, K=128, bias=None, out=P,
+             o_sm=10)
+    a.update(change)
+    L = _hip.lib()
+    assert L.coda_linear_int8(*a.values(), None) == 1
+    assert error in L.coda_last_error().decode()
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(dtype=2), "dtype"), (dict(Dh=6), "sizes"), (dict(M=-1), "sizes"), (dict(q=None), "missing"),
+    (dict(bias=P + 4), "16-byte"), (dict(g=None), "missing"), (dict(k=P + 2), "8-byte"), (dict(x_sm=100), "16-byte"),
+])
+def test_project_entry(change, error):
+    d = _hip.ProjDesc()
+    for n, v in dict(dict(dtype=1, M=2, L=1, H=2, Hkv=1, Dh=64, gate=1, x=P, x_sm=128, w=P, bias=P, rope_cos=P, rope_sin=P,
+                          q=P, q_sm=128, k=P, k_sm=64, v=P, v_sm=64, lam=P, lam_sm=2, g=P), **change).items():
+        setattr(d, n, v)
+    L = _hip.lib()
+    assert L.coda_project_int8(d, P, P, 128, 128, None) == 1
+    assert error in L.coda_last_error().decode()
+    assert L.coda_project_int8(None, P, P, 128, 128, None) == 1
