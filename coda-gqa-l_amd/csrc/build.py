@@ -31,11 +31,12 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
          # no implicit multiply-add fusion: the reference rounds every product
          # before the add; accumulations that want FMA call fmaf explicitly
          "-ffp-contract=off",
-         # MFMA accumulators in ordinary VGPRs: the online-softmax rescale and
-         # the epilogue read them with VALU instructions, which cannot address
-         # AGPRs (every access would be a copy)
-         "-mllvm", "-amdgpu-mfma-vgpr-form",
          "-Wno-unused-result"]
+# MFMA accumulators in ordinary VGPRs: the online-softmax rescale and the
+# epilogue read them with VALU instructions, which cannot address AGPRs (every
+# access would be a copy).  Not for int8.hip: a wave of its largest tile has
+# 256 accumulators, which read nothing until the end and fill the AGPRs.
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 
 
 def hipcc() -> str:
@@ -47,7 +48,8 @@ def hipcc() -> str:
 
 def _compile(src: str, tag: str) -> str:
     obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
-    cmd = [hipcc(), *FLAGS, f'-DCODA_SOURCE_HASH="{tag}"', "-c", os.path.join(HERE, src), "-o", obj]
+    flags = FLAGS if src == "int8.hip" else FLAGS + VGPR_FORM
+    cmd = [hipcc(), *flags, f'-DCODA_SOURCE_HASH="{tag}"', "-c", os.path.join(HERE, src), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in (r.stderr or "").splitlines() if noise not in l)

@@ -9,6 +9,7 @@
 
 #include <climits>
 #include <type_traits>
+#include <utility>
 
 namespace coda {
 
@@ -183,22 +184,12 @@ __global__ __launch_bounds__(256) void values_kernel(const int8_t* __restrict__ 
 }
 
 // ------------------------------------------------------------ product
+//   y[m, f] = round_T((sum_k x[m, k] w[f, k]) sx[m] sw[f] + bias[f])
+// with the sum exact in int32 (so that neither the tile nor a split of K
+// shows in the result).  MFMA rows (operand A) are the features, columns (B)
+// the tokens: a lane holds four consecutive features of a token.
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-
-// Epilogue of a plain product: out = value + bias, one rounding
-template <typename T>
-struct Int8Out {
-  T* out;
-  const T* bias;  // or null
-  int64_t o_sm;
-  int n_feat;
-  __device__ __forceinline__ void operator()(const int&, int f, int m, pf32x4 v) const {
-    T* row = out + (int64_t)m * o_sm;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (f + e < n_feat) row[f + e] = Elt<T>::st(bias ? v[e] + Elt<T>::ld(bias[f + e]) : v[e]);
-  }
-};
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 struct Int8Mat {
   const int8_t* p;
@@ -207,51 +198,264 @@ struct Int8Mat {
   int rows;
 };
 
-// y[m, f] = (sum_k x[m, k] w[f, k]) sx[m] sw[f], the sum exact in int32, then
-// the epilogue.  A workgroup of 4 waves makes 64 features x 64 tokens, a wave
-// 16 x 64; the MFMA's rows are the features, so a lane holds four consecutive
-// ones of a token.
-template <typename Epi>
-__global__ __launch_bounds__(256) void int8_tile64(const Int8Mat X, const Int8Mat W, int K, int ntf, const Epi epi) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
-  const int f0 = (blockIdx.x % ntf) * 64 + 16 * wv, m0 = (int)(blockIdx.x / ntf) * 64;
-  const int8_t* wr = W.p + (int64_t)min(f0 + r16, W.rows - 1) * W.sm + 16 * kq;
-  const int8_t* xr[4];
+// four features of a token, rounded to T
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+
+// Where the values of a product go: bias1(f) what is added to feature f;
+// lane(f) what a lane that writes features f .. f + 3 (a multiple of 4) of
+// several tokens needs to know once; put() writes them for token m.
+template <typename T>
+struct LinearSink {
+  typedef T Out;
+  T* out;
+  const T* bias;  // or null
+  int64_t o_sm;
+  int n_feat;
+  struct Lane {
+    T* p;
+    int n;
+  };
+  __device__ __forceinline__ float bias1(int f) const { return bias ? Elt<T>::ld(bias[f]) : 0.f; }
+  __device__ __forceinline__ Lane lane(int f) const { return Lane{out + f, n_feat - f}; }
+  __device__ __forceinline__ void put(const Lane& l, int m, const Four<T>& v) const {
+    // (rows of any element address)
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef typename std::conditional<sizeof(T) == 2, u16x4, u32x4>::type V;
+    T* row = l.p + (int64_t)m * o_sm;
+    if (l.n >= 4) {
+      *reinterpret_cast<V*>(row) = __builtin_bit_cast(V, v);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) xr[j] = X.p + (int64_t)min(m0 + 16 * j + r16, X.rows - 1) * X.sm + 16 * kq;
-  i32x4 acc[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = i32x4{0, 0, 0, 0};
-  for (int k = 0; k < K; k += 64) {
-    const i32x4 a = *reinterpret_cast<const i32x4*>(wr + k);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *reinterpret_cast<const i32x4*>(xr[j] + k), acc[j], 0, 0, 0);
+      for (int e = 0; e < 3; ++e)
+        if (e < l.n) row[e] = v.v[e];
+    }
   }
-  const int f = f0 + 4 * kq;
-  if (f >= W.rows) return;
-  float sw[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sw[e] = W.scales[min(f + e, W.rows - 1)];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = m0 + 16 * j + r16;
-    if (m >= X.rows) continue;
-    const float sx = X.scales[m];
-    pf32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][e] * sx * sw[e];
-    epi(0, f, m, v);
+};
+
+// The projection front end (FrontEpilogue, its bias added already)
+struct NoBias {
+  __device__ __forceinline__ pf32x4 bias4(int, int) const { return pf32x4{0.f, 0.f, 0.f, 0.f}; }
+};
+template <typename T>
+struct FrontSink {
+  typedef T Out;
+  FrontEpilogue<T, true> epi;
+  int n_feat;
+  struct Lane {
+    int f;
+  };
+  __device__ __forceinline__ float bias1(int f) const { return epi.d.bias[f]; }
+  __device__ __forceinline__ Lane lane(int f) const { return Lane{f}; }
+  __device__ __forceinline__ void put(const Lane& l, int m, const Four<T>& v) const {
+    using E = Elt<T>;
+    epi(NoBias{}, l.f, m, pf32x4{E::ld(v.v[0]), E::ld(v.v[1]), E::ld(v.v[2]), E::ld(v.v[3])});
   }
+};
+
+template <typename T>
+__device__ __forceinline__ Four<T> int8_value(const i32x4& a, float sx, const pf32x4& sw, const pf32x4& bias) {
+  Four<T> v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v.v[e] = Elt<T>::st((float)a[e] * sx * sw[e] + bias[e]);
+  return v;
 }
 
-template <typename Epi>
-static int launch_int8(const Int8Mat& X, const Int8Mat& W, int K, const Epi& epi, hipStream_t st) {
-  const int ntf = (W.rows + 63) / 64;
-  const int64_t n = (int64_t)ntf * ((X.rows + 63) / 64);
-  if (n > INT_MAX) return fail(CODA_EUNSUP, "int8 product: %lld tiles", (long long)n);
-  hipLaunchKernelGGL((int8_tile64<Epi>), dim3((unsigned)n), dim3(256), 0, st, X, W, K, ntf, epi);
-  return check_launch("int8_tile64");
+// ---- tiles
+// 16 bytes a lane, global -> LDS at lds + 16 lane (counted in vmcnt)
+__device__ __forceinline__ void tile_load16(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ uint32_t tile_lds(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+// LDS read by hand: the compiler would wait for every load to LDS in flight
+// before its own (it cannot tell the stages apart)
+template <int OFF>
+__device__ __forceinline__ i32x4 tile_read(uint32_t addr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset is 16 bits");
+  i32x4 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF));
+  return r;
+}
+// all of its reads have landed
+template <int N>
+__device__ __forceinline__ void tile_landed(i32x4 (&a)[N]) {
+  if constexpr (N == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]));
+  if constexpr (N == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+  if constexpr (N == 8)
+    asm volatile("s_waitcnt lgkmcnt(0)"
+                 : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7]));
+}
+template <class F, int... I>
+__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// 4 waves (2 x 2) make 64 S features x 64 S tokens, a wave 32 S x 32 S in
+// S x S accumulators of 32 x 32.  K passes through LDS in steps of 64 bytes,
+// four stages: while the products of step k run, step k + 1 lies in LDS
+// (its first operands are read ahead, so that no product waits for LDS after
+// a barrier), step k + 2 is on its way and step k + 3 is asked for: one
+// barrier a step.  A stage holds a row's four 16-byte pieces in the order
+// slot = piece ^ (row / 2) % 4, by which eight lanes that read one piece of
+// eight rows touch every bank once.
+template <int S>
+struct TileLds {
+  static constexpr int kRows = 128 * S;       // features, then tokens
+  static constexpr int kStage = kRows * 64;   // bytes
+  static constexpr int kStages = 4;
+  static constexpr size_t kBytes = (size_t)kStages * kStage;
+};
+template <int S, typename Sink>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 : 2))) void int8_tile(
+    const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
+  typedef typename Sink::Out T;
+  typedef TileLds<S> L;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int BF = 64 * S, BM = 64 * S, NL = L::kRows / 64;  // loads a thread and step
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
+  // in groups of 4 token tiles, so that what it has at a time shares rows in
+  // its L2.
+  const int n = ntf * ntm, xcd = blockIdx.x & 7, base = n >> 3, rem = n & 7;
+  const int t = xcd * base + min(xcd, rem) + (int)(blockIdx.x >> 3);
+  const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
+  const int f0 = in / gm * BF, m0 = (4 * group + in % gm) * BM;
+  // this lane's pieces: rows of a load are 16, four pieces each
+  const int8_t* src[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int r = (4 * i + wv) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 1) & 3);
+    src[i] = r < BF ? W.p + (int64_t)min(f0 + r, W.rows - 1) * W.sm + 16 * piece
+                    : X.p + (int64_t)min(m0 + r - BF, X.rows - 1) * X.sm + 16 * piece;
+  }
+  const int steps = K / 64;
+  auto load = [&](int k) {
+    char* st = smem + (k & 3) * L::kStage + wv * 1024;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) tile_load16(src[i] + (int64_t)k * 64, st + i * 4096);
+  };
+  i32x16 acc[S][S];
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  // operands of half h of a step: pieces 2 h + lane / 32
+  const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
+  const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 1) & 3)) << 4);
+  i32x4 op[2][2 * S];
+  auto read = [&](auto c, i32x4 (&o)[2 * S], uint32_t a) {  // operand c: S of features, S of tokens
+    constexpr int i = decltype(c)::value;
+    o[i] = i < S ? tile_read<i * 2048>(a + wf * (S * 2048)) : tile_read<BF * 64 + (i - S) * 2048>(a + wm * (S * 2048));
+  };
+  // products of one half, and meanwhile the reads of the next
+  auto half = [&](i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a) {
+    each<S * S>([&](auto c) {
+      constexpr int q = decltype(c)::value, i = q / S, j = q % S;
+      // (2 S reads beside the first half of the products)
+      constexpr int per = S == 1 ? 2 : S == 2 ? 2 : 1;
+      each<per>([&](auto d) {
+        constexpr int k = q * per + decltype(d)::value;
+        if constexpr (k < 2 * S) read(std::integral_constant<int, k>{}, next, a);
+      });
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[S + j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    tile_landed(next);
+  };
+  // (K is a multiple of 128: two steps at least)
+  load(0);
+  load(1);
+  if (steps > 2) load(2);
+  __builtin_amdgcn_sched_barrier(0);
+  // steps 0 and 1 have landed
+  if (steps > 2) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
+  else __builtin_amdgcn_s_waitcnt(0x0f70);
+  __builtin_amdgcn_s_barrier();
+  each<2 * S>([&](auto c) { read(c, op[0], at); });
+  tile_landed(op[0]);
+  for (int k = 0; k < steps; ++k) {
+    // here: step k + 1 has landed for every wave, all have done with k - 1
+    if (k + 3 < steps) load(k + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t here = at + (k & 3) * L::kStage;
+    // (past the last step: its own operands again)
+    const uint32_t then = at + (min(k + 1, steps - 1) & 3) * L::kStage;
+    half(op[0], op[1], here ^ 32);
+    half(op[1], op[0], then);
+    if (k + 3 < steps) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);  // step k + 2 has landed
+    else __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Values pass through LDS (a wave's own part) from four features of 32
+  // tokens a lane to runs of a token's features, 32 tokens at a time; the
+  // features' scales and biases lie there too
+  constexpr int ROW = 32 * S * sizeof(T) + 16, QR = 8 * S;  // bytes of a row, fours of features in it
+  float* fs = reinterpret_cast<float*>(smem);
+  if (threadIdx.x < BF) {
+    const int f = min(f0 + (int)threadIdx.x, W.rows - 1);
+    fs[threadIdx.x] = W.scales[f];
+    fs[BF + threadIdx.x] = sink.bias1(f);
+  }
+  __syncthreads();
+  char* mine = smem + 2 * BF * sizeof(float) + wv * 32 * ROW;
+  const int fw = f0 + 32 * S * wf, mw = m0 + 32 * S * wm, q = lane % QR, fq = fw + 4 * q;
+  const typename Sink::Lane to = sink.lane(min(fq, W.rows - 1));
+  const char* own = smem + (32 * S * wf + 4 * (lane >> 5)) * sizeof(float);
+  each<S>([&](auto jc) {
+    constexpr int j = decltype(jc)::value;
+    const float sx = X.scales[min(mw + 32 * j + r32, X.rows - 1)];
+    each<4 * S>([&](auto gc) {
+      constexpr int i = decltype(gc)::value / 4, g = decltype(gc)::value % 4, fl = 32 * i + 8 * g;
+      const pf32x4 sw = *reinterpret_cast<const pf32x4*>(own + fl * sizeof(float));
+      const pf32x4 bias = *reinterpret_cast<const pf32x4*>(own + (BF + fl) * sizeof(float));
+      const i32x4 a{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      *reinterpret_cast<Four<T>*>(mine + r32 * ROW + (fl + 4 * (lane >> 5)) * sizeof(T)) = int8_value<T>(a, sx, sw, bias);
+    });
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+    for (int r = 0; r < 32; r += 64 / QR) {
+      const int row = r + lane / QR, m = mw + 32 * j + row;
+      const Four<T> v = *reinterpret_cast<const Four<T>*>(mine + row * ROW + q * 4 * sizeof(T));
+      if (m < X.rows && fq < W.rows) sink.put(to, m, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+  });
+}
+
+template <int S, typename Sink>
+static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
+  typedef TileLds<S> L;
+  const int64_t ntf = ((int64_t)W.rows + 64 * S - 1) / (64 * S), ntm = ((int64_t)X.rows + 64 * S - 1) / (64 * S);
+  if (ntf * ntm > INT_MAX) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)(ntf * ntm));
+  constexpr size_t values = (size_t)2 * 64 * S * 4 + 4 * 32 * (32 * S * sizeof(typename Sink::Out) + 16);
+  constexpr size_t lds = values > L::kBytes ? values : L::kBytes;
+  const int rc = lds_limit<int8_tile<S, Sink>>(lds, who);
+  if (rc) return rc;
+  hipLaunchKernelGGL((int8_tile<S, Sink>), dim3((unsigned)(ntf * ntm)), dim3(256), lds, st, X, W, K, (int)ntf, (int)ntm,
+                     sink);
+  return check_launch("int8_tile");
+}
+
+template <typename Sink>
+static int launch_int8(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
+  // the largest tile that gives every CU one
+  const int cus = device_cus();
+  auto tiles = [&](int b) { return ((int64_t)W.rows + b - 1) / b * (((int64_t)X.rows + b - 1) / b); };
+  if (tiles(256) >= cus) return launch_tile<4>(X, W, K, sink, st, who);
+  if (tiles(128) >= cus) return launch_tile<2>(X, W, K, sink, st, who);
+  return launch_tile<1>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {
@@ -338,7 +542,7 @@ extern "C" int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const 
   if (rc || M == 0) return rc;
   CODA_REQUIRE(out && o_sm >= n_feat, "%s: no output, or its rows shorter than %d features", who, n_feat);
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T) launch_int8(X, W, K, Int8Out<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st)
+#define RUN(T) launch_int8(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who)
   return dtype == CODA_F32 ? RUN(float) : dtype == CODA_BF16 ? RUN(bf16_t) : RUN(f16_t);
 #undef RUN
 }
@@ -361,6 +565,7 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
                    ((uintptr_t)d->k % 8) == 0 && ((uintptr_t)d->v % 8) == 0,
                "%s: q / k / v rows must be 8-byte aligned", who);
   const hipStream_t st = (hipStream_t)stream;
-  return d->dtype == CODA_BF16 ? launch_int8(X, W, K, FrontEpilogue<bf16_t, false>{*d, FrontTables{}}, st)
-                               : launch_int8(X, W, K, FrontEpilogue<float, false>{*d, FrontTables{}}, st);
+#define RUN(T) launch_int8(X, W, K, FrontSink<T>{{*d, FrontTables{}}, n_feat}, st, who)
+  return d->dtype == CODA_BF16 ? RUN(bf16_t) : RUN(float);
+#undef RUN
 }
