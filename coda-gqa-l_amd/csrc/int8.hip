@@ -5,10 +5,9 @@
 // value of a code being code * scale.  A row's codes lie at a 16-byte address
 // and are followed by zeros up to a multiple of kPad bytes, so that the
 // product runs over whole 128-byte steps and has no ragged end.
-#include "front.h"
+#include "rows.h"
 
 #include <climits>
-#include <type_traits>
 #include <utility>
 
 namespace coda {
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(256) void values_kernel(const int8_t* __restrict__ 
 // with the sum exact in int32 (so that neither the tile nor a split of K
 // shows in the result).  MFMA rows (operand A) are the features, columns (B)
 // the tokens: a lane holds four consecutive features of a token.
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef pi32x4 i32x4;
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 struct Int8Mat {
@@ -448,8 +447,32 @@ static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   return check_launch("int8_tile");
 }
 
+// ---- few token rows: the row kernels of the float projections on codes
+template <typename Sink>
+struct RowsSink {
+  Sink sink;
+  const float* sx;
+  const float* sw;
+  int n_feat;
+  template <typename Src>
+  __device__ __forceinline__ void operator()(const Src&, int f, int m, const i32x4& a) const {
+    pf32x4 s, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int g = min(f + e, n_feat - 1);
+      s[e] = sw[g];
+      b[e] = sink.bias1(g);
+    }
+    sink.put(sink.lane(f), m, int8_value<typename Sink::Out>(a, sx[m], s, b));
+  }
+  __device__ __forceinline__ void once(int) const {}
+};
+
 template <typename Sink>
 static int launch_int8(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
+  if (X.rows <= 128)
+    return launch_rows<int8_t>(MatRows<int8_t>{W.p, W.sm}, W.rows, K, X.p, X.sm, X.rows,
+                               RowsSink<Sink>{sink, X.scales, W.scales, W.rows}, st, who);
   // the largest tile that gives every CU one
   const int cus = device_cus();
   auto tiles = [&](int b) { return ((int64_t)W.rows + b - 1) / b * (((int64_t)X.rows + b - 1) / b); };
