@@ -14,8 +14,6 @@ as RuntimeError, like those of the other operators.
 
 from __future__ import annotations
 
-import contextlib
-from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
@@ -32,14 +30,6 @@ def _padded(cols: int) -> int:
     return -(-cols // PAD) * PAD
 
 
-def _on(t: torch.Tensor):
-    """Work on t's device, whichever is current."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-@dataclass(frozen=True)
 class Int8Rows:
     """Rows of 8-bit codes: the value at (row, c) is codes[row, c] *
     scales[row].
@@ -50,21 +40,20 @@ class Int8Rows:
     held an infinity or a NaN) makes NaN of all that is computed from it.
     from_codes() lays out codes of the plain shape (..., cols)."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    cols: int
-    dtype: torch.dtype
+    __slots__ = ("codes", "scales", "cols", "dtype")
 
-    def __post_init__(self):
-        c, s = self.codes, self.scales
-        if c.dtype != torch.int8 or s.dtype != torch.float32:
-            raise RuntimeError(f"Int8Rows: codes must be int8 and scales float32, got {c.dtype} and {s.dtype}")
-        if self.cols <= 0 or c.dim() < 1 or c.shape[-1] != _padded(self.cols):
-            raise RuntimeError(f"Int8Rows: codes {tuple(c.shape)} for rows of {self.cols}: the last size must be "
-                               f"{_padded(max(int(self.cols), 1))} (from_codes() lays out plain codes)")
-        if s.shape != c.shape[:-1] or s.device != c.device:
-            raise RuntimeError(f"Int8Rows: scales {tuple(s.shape)} on {s.device} for codes {tuple(c.shape)} on {c.device}")
-        _hip.dtype_code(self.dtype)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype):
+        if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
+            raise RuntimeError(f"Int8Rows: codes must be int8 and scales float32, got {codes.dtype} and {scales.dtype}")
+        shape = codes.shape
+        if cols <= 0 or not shape or shape[-1] != _padded(cols):
+            raise RuntimeError(f"Int8Rows: codes {tuple(shape)} for rows of {cols}: the last size must be "
+                               f"{_padded(max(int(cols), 1))} (from_codes() lays out plain codes)")
+        if scales.shape != shape[:-1] or scales.device != codes.device:
+            raise RuntimeError(f"Int8Rows: scales {tuple(scales.shape)} on {scales.device} for codes {tuple(shape)} on "
+                               f"{codes.device}")
+        _hip.dtype_code(dtype)
+        self.codes, self.scales, self.cols, self.dtype = codes, scales, int(cols), dtype
 
     @staticmethod
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> "Int8Rows":
@@ -89,39 +78,76 @@ class Int8Rows:
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The values, in `dtype` (None: the rows' own)."""
         dtype = self.dtype if dtype is None else dtype
-        codes, scales = _flat(self)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(codes):
-            _hip.check(_hip.lib().coda_dequantize_rows(
-                _hip.dtype_code(dtype), codes.data_ptr(), codes.stride(0), scales.data_ptr(), codes.shape[0], self.cols,
-                out.data_ptr(), self.cols, _hip.stream_of(codes)))
+        code = _hip.dtype_code(dtype)
+        codes, sm, scales = _flat(self)
+        out = torch.empty(self.shape, dtype=dtype, device=codes.device)
+        _call(_hip.lib().coda_dequantize_rows, codes, code, codes.data_ptr(), sm, scales.data_ptr(), scales.numel(),
+              self.cols, out.data_ptr(), self.cols)
         return out
 
 
-def _flat(r: Int8Rows) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(codes (rows, P) whose rows lie at 16-byte addresses, scales (rows,)
-    without gaps), copied only where they do not lie so."""
-    _hip.require_device(r.codes, r.scales)
-    c = r.codes.reshape(-1, r.codes.shape[-1])
-    if c.stride(1) != 1 or c.stride(0) % 16 or c.data_ptr() % 16:
-        c = c.clone(memory_format=torch.contiguous_format)
-    return c, r.scales.reshape(-1).contiguous()
+def _made(codes: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype) -> Int8Rows:
+    """Int8Rows of codes that this module has laid out."""
+    r = Int8Rows.__new__(Int8Rows)
+    r.codes, r.scales, r.cols, r.dtype = codes, scales, cols, dtype
+    return r
 
 
-def _rows_of(x: torch.Tensor) -> torch.Tensor:
-    """x (..., D) as (rows, D) with unit stride over D."""
-    x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
+# the current stream's address, without the Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _new_rows(x: torch.Tensor, D: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    lead = x.shape[:-1]
-    return (torch.empty((*lead, _padded(D)), dtype=torch.int8, device=x.device),
-            torch.empty(lead, dtype=torch.float32, device=x.device))
+def _call(fn, t: torch.Tensor, *args) -> None:
+    """A library call on t's device, whichever is current, and its current
+    stream."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _hip.check(rc)
+
+
+def _flat(r: Int8Rows) -> Tuple[torch.Tensor, int, torch.Tensor]:
+    """(codes whose rows lie at 16-byte addresses, bytes from one to the next,
+    scales without gaps), copied only where they do not lie so."""
+    c, s = r.codes, r.scales
+    if not c.is_cuda:
+        _hip.require_device(c, s)
+    if not s.is_contiguous():
+        s = s.contiguous()
+    if not c.is_contiguous():
+        c = c.reshape(-1, c.shape[-1])
+        if c.stride(1) == 1 and c.stride(0) % 16 == 0 and c.data_ptr() % 16 == 0:
+            return c, c.stride(0), s
+        c = c.contiguous()
+    if c.data_ptr() % 16:
+        c = c.clone()
+    return c, c.shape[-1], s
+
+
+def _rows_of(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """x (..., D) with unit stride over D, and the elements from one row to
+    the next."""
+    D = x.shape[-1]
+    if x.is_contiguous():
+        return x, D
+    x = x.reshape(-1, D)
+    return (x, x.stride(0)) if x.stride(1) == 1 or D == 1 else (x.contiguous(), D)
+
+
+def _new_rows(x: torch.Tensor, D: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
+    """Uninitialised codes and scales of x's rows, and the codes of a row."""
+    lead, P, dev = x.shape[:-1], _padded(D), x.device
+    return torch.empty((*lead, P), dtype=torch.int8, device=dev), torch.empty(lead, dtype=torch.float32, device=dev), P
 
 
 def _check_input(x: torch.Tensor, who: str) -> int:
-    _hip.require_device(x)
+    if not x.is_cuda:
+        _hip.require_device(x)
     if x.dim() < 1 or not 0 < x.shape[-1] <= MAX_ROW:
         raise RuntimeError(f"{who}: rows of 1 to {MAX_ROW} elements, got {tuple(x.shape)}")
     return x.shape[-1]
@@ -132,13 +158,13 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     the nearest to x / scale (ties to even).  For a weight (out, in) the rows
     are its output channels.  D at most 32768."""
     D = _check_input(x, "quantize_rows")
-    x2 = _rows_of(x.detach())
-    codes, scales = _new_rows(x, D)
-    with _on(x):
-        _hip.check(_hip.lib().coda_quantize_rows(
-            _hip.dtype_code(x.dtype), x2.data_ptr(), x2.stride(0), x2.shape[0], D, codes.data_ptr(), codes.shape[-1],
-            scales.data_ptr(), _hip.stream_of(x)))
-    return Int8Rows(codes, scales, D, x.dtype)
+    dt = x.dtype
+    code = _hip.dtype_code(dt)
+    x2, sm = _rows_of(x)
+    codes, scales, P = _new_rows(x, D)
+    _call(_hip.lib().coda_quantize_rows, x, code, x2.data_ptr(), sm, scales.numel(), D, codes.data_ptr(), P,
+          scales.data_ptr())
+    return _made(codes, scales, D, dt)
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None
@@ -149,29 +175,30 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     next sublayer.  x, weight (D,) and residual share their type; D at most
     32768."""
     D = _check_input(x, "rms_norm_int8")
-    _hip.require_device(weight, residual)
-    if tuple(weight.shape) != (D,):
+    dt = x.dtype
+    code = _hip.dtype_code(dt)
+    if weight.shape != (D,):
         raise RuntimeError(f"rms_norm_int8: weight {tuple(weight.shape)}, expected ({D},)")
     if residual is not None and residual.shape != x.shape:
         raise RuntimeError(f"rms_norm_int8: residual {tuple(residual.shape)} is not x's shape {tuple(x.shape)}")
     for name, t in (("weight", weight), ("residual", residual)):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise RuntimeError(f"rms_norm_int8: {name} is {t.dtype} on {t.device}, x {x.dtype} on {x.device}")
+        if t is not None and (t.dtype is not dt or t.device != x.device):
+            raise RuntimeError(f"rms_norm_int8: {name} is {t.dtype} on {t.device}, x {dt} on {x.device}")
     if not eps >= 0:
         raise RuntimeError(f"rms_norm_int8: eps={eps} is negative")
-    x2, w = _rows_of(x.detach()), weight.detach().contiguous()
-    codes, scales = _new_rows(x, D)
-    r2 = out = None
-    if residual is not None:
-        r2 = _rows_of(residual.detach())
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _on(x):
-        _hip.check(_hip.lib().coda_rms_norm_int8(
-            _hip.dtype_code(x.dtype), x2.data_ptr(), x2.stride(0), _hip.ptr(r2), 0 if r2 is None else r2.stride(0),
-            w.data_ptr(), x2.shape[0], D, float(eps), _hip.ptr(out), D, codes.data_ptr(), codes.shape[-1],
-            scales.data_ptr(), _hip.stream_of(x)))
-    rows = Int8Rows(codes, scales, D, x.dtype)
-    return rows if residual is None else (rows, out)
+    x2, sm = _rows_of(x)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    codes, scales, P = _new_rows(x, D)
+    fn = _hip.lib().coda_rms_norm_int8
+    if residual is None:
+        _call(fn, x, code, x2.data_ptr(), sm, None, 0, w.data_ptr(), scales.numel(), D, float(eps), None, 0,
+              codes.data_ptr(), P, scales.data_ptr())
+        return _made(codes, scales, D, dt)
+    r2, rm = _rows_of(residual)
+    out = torch.empty(x.shape, dtype=dt, device=x.device)
+    _call(fn, x, code, x2.data_ptr(), sm, r2.data_ptr(), rm, w.data_ptr(), scales.numel(), D, float(eps),
+          out.data_ptr(), D, codes.data_ptr(), P, scales.data_ptr())
+    return _made(codes, scales, D, dt), out
 
 
 def linear_int8(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -180,19 +207,18 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
     (N,), rounded once to x's type.  K at most 130944."""
     if not isinstance(x, Int8Rows) or not isinstance(weight, Int8Rows):
         raise TypeError("linear_int8 takes Int8Rows (quantize_rows, rms_norm_int8 make them)")
-    if weight.codes.dim() != 2 or weight.cols != x.cols or weight.codes.shape[0] == 0:
+    wc, dt = weight.codes, x.dtype
+    if wc.dim() != 2 or weight.cols != x.cols or wc.shape[0] == 0:
         raise RuntimeError(f"linear_int8: weight {tuple(weight.shape)} does not fit x {tuple(x.shape)}")
-    N = weight.codes.shape[0]
-    _hip.require_device(x.codes, weight.codes, bias)
-    if weight.device != x.device or bias is not None and (bias.device != x.device or bias.dtype != x.dtype or
-                                                          tuple(bias.shape) != (N,)):
+    N, P = wc.shape
+    a, am, sa = _flat(x)
+    b, bm, sb = _flat(weight)
+    dev = a.device
+    if b.device != dev or bias is not None and (bias.device != dev or bias.dtype is not dt or bias.shape != (N,)):
         raise RuntimeError("linear_int8: weight and bias must be on x's device, bias (N,) of x's type")
-    a, sa = _flat(x)
-    b, sb = _flat(weight)
-    bias = None if bias is None else bias.detach().contiguous()
-    out = torch.empty((*x.codes.shape[:-1], N), dtype=x.dtype, device=x.device)
-    with _on(a):
-        _hip.check(_hip.lib().coda_linear_int8(
-            _hip.dtype_code(x.dtype), a.data_ptr(), a.stride(0), sa.data_ptr(), a.shape[0], b.data_ptr(), b.stride(0),
-            sb.data_ptr(), N, b.shape[1], _hip.ptr(bias), out.data_ptr(), N, _hip.stream_of(a)))
+    if bias is not None:
+        bias = bias.contiguous()
+    out = torch.empty((*x.codes.shape[:-1], N), dtype=dt, device=dev)
+    _call(_hip.lib().coda_linear_int8, a, _hip.dtype_code(dt), a.data_ptr(), am, sa.data_ptr(), sa.numel(), b.data_ptr(),
+          bm, sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
     return out

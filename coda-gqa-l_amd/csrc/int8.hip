@@ -28,6 +28,41 @@ __device__ __forceinline__ double wave_reduce(double v, bool max) {
   return v;
 }
 
+// a run of 8 elements, at any element address
+template <typename T>
+struct Run8 {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Run8<T> run_ld(const T* p, int n) {  // elements past n: 0
+  Run8<T> r;
+  if (n >= 8) {
+    constexpr int N = sizeof(Run8<T>) / 16;
+    pu32x4 w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const pu32x4u*>(p)[i];
+    __builtin_memcpy(&r, w, sizeof(r));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = e < n ? p[e] : Elt<T>::st(0.f);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void run_st(T* p, int n, const Run8<T>& r) {
+  if (n >= 8) {
+    constexpr int N = sizeof(Run8<T>) / 16;
+    pu32x4 w[N];
+    __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<pu32x4u*>(p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = r.v[e];
+  }
+}
+
 // Rows in 8 bits, with p_i = x_i (plain) or p_i = s_i w_i (norm; s = x +
 // residual, rounded to T and written):
 //   P = max |p|, code_i = rint(127 p_i / P),
@@ -35,151 +70,186 @@ __device__ __forceinline__ double wave_reduce(double v, bool max) {
 // the norm is the same factor for the whole row, so the codes need not wait
 // for it.  p, P, the sum and the quotient are held in 64 bits: a product of
 // two floats is exact there, and a quotient that falls on a half is rounded
-// to even as the formula says, whatever the order of the sums.  A row that
-// holds an infinity or a NaN (its weight's counts too) gets scale NaN and
-// codes 0; a row of zeros scale 0.
-// TPR threads keep a row in registers (IT runs of VEC elements each) between
+// to even as the formula says, whatever the order of the sums.  (Plain rows
+// of 16 bits: p and P need no more than fp32, and the quotient's remainder,
+// of at most 18 bits, is exact in it.)  A row that holds an infinity or a
+// NaN (its weight's count too) gets scale NaN and codes 0; a row of zeros
+// scale 0.
+// TPR threads keep a row in registers (IT runs of 8 elements each) between
 // the row's maximum and its codes, so that memory is read once.
-template <typename T, bool NORM, bool RES, int VEC, int TPR, int IT>
+template <typename T, bool NORM, bool RES, int TPR, int IT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void codes_kernel(
     const T* __restrict__ x, int64_t x_sm, const T* __restrict__ res, int64_t r_sm, const T* __restrict__ w, int rows,
     int D, float eps, T* __restrict__ sum_out, int64_t s_sm, int8_t* __restrict__ codes, int64_t c_sm,
     float* __restrict__ scales) {
   using E = Elt<T>;
+  // the type of p and of the quotient, and the shift that leaves a quotient's
+  // nearest integer (ties to even) in its low bits: 1.5 times 2^23 or 2^52
+  typedef typename std::conditional<!NORM && sizeof(T) == 2, float, double>::type R;
+  constexpr R kShift = sizeof(R) == 4 ? (R)12582912. : (R)6755399441055744.;
   constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-  struct alignas(sizeof(T) * VEC) Run { T v[VEC]; };
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   if (TPR == 64 && row >= rows) return;  // (whole waves; else a workgroup is a row)
   const T* xr = x + row * x_sm;
-  double p[IT * VEC];
-  double ss = 0., top = 0., bad = 0.;
+  R p[IT * 8];
+  double ss = 0.;
+  R top = 0, bad = 0;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int at = (i * TPR + t) * VEC;
+    const int at = (i * TPR + t) * 8, n = D - at;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) p[i * VEC + e] = 0.;
-    if (at >= D) continue;
-    Run a = *reinterpret_cast<const Run*>(xr + at);
+    for (int e = 0; e < 8; ++e) p[i * 8 + e] = 0;
+    if (n <= 0) continue;
+    Run8<T> a = run_ld(xr + at, n);
     if constexpr (NORM) {
-      const Run g = *reinterpret_cast<const Run*>(w + at);
+      const Run8<T> g = run_ld(w + at, n);
       if constexpr (RES) {
-        const Run r = *reinterpret_cast<const Run*>(res + row * r_sm + at);
+        const Run8<T> r = run_ld(res + row * r_sm + at, n);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a.v[e] = E::st(E::ld(a.v[e]) + E::ld(r.v[e]));
-        *reinterpret_cast<Run*>(sum_out + row * s_sm + at) = a;
+        for (int e = 0; e < 8; ++e) a.v[e] = E::st(E::ld(a.v[e]) + E::ld(r.v[e]));
+        run_st(sum_out + row * s_sm + at, n, a);
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const double s = (double)E::ld(a.v[e]);
         ss = fma(s, s, ss);
-        p[i * VEC + e] = s * (double)E::ld(g.v[e]);
+        p[i * 8 + e] = s * (double)E::ld(g.v[e]);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) p[i * VEC + e] = (double)E::ld(a.v[e]);
+      for (int e = 0; e < 8; ++e) p[i * 8 + e] = (R)E::ld(a.v[e]);
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      top = fmax(top, fabs(p[i * VEC + e]));
-      bad = fma(p[i * VEC + e], 0., bad);  // NaN from an infinity or a NaN
+    for (int e = 0; e < 8; ++e) {
+      top = __builtin_elementwise_max(top, __builtin_elementwise_abs(p[i * 8 + e]));
+      bad = __builtin_elementwise_fma(p[i * 8 + e], (R)0, bad);  // NaN from an infinity or a NaN
     }
   }
   ss += bad;
   ss = wave_reduce(ss, false);
-  top = wave_reduce(top, true);
+  double P = wave_reduce((double)top, true);
   if constexpr (TPR > 64) {
     constexpr int NW = TPR / 64;
     __shared__ double red[2][NW];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     if (lane == 0) {
       red[0][wv] = ss;
-      red[1][wv] = top;
+      red[1][wv] = P;
     }
     __syncthreads();
     ss = red[0][0];
-    top = red[1][0];
+    P = red[1][0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) {
       ss += red[0][i];
-      top = fmax(top, red[1][i]);
+      P = fmax(P, red[1][i]);
     }
   }
-  const bool fine = ss == ss && top > 0.;
-  const double r = fine ? 1. / top : 0.;
+  const bool fine = ss == ss && P > 0.;
   if (t == 0) {
-    double sc = top / 127.;
+    double sc = P / 127.;
     if constexpr (NORM) sc /= sqrt(ss / (double)D + (double)eps);
-    scales[row] = ss != ss ? __builtin_nanf("") : top > 0. ? (float)sc : 0.f;
+    scales[row] = ss != ss ? __builtin_nanf("") : P > 0. ? (float)sc : 0.f;
+  }
+  // 127 p / P to the last bit: n = 127 p, the quotient by the reciprocal, then
+  // its remainder's share.  In fp32 P is brought to [1, 2) (p by the same
+  // power of two), where neither leaves the range.
+  R k = 127, Q = (R)P, inv = 0;
+  if (fine) {
+    if constexpr (sizeof(R) == 4) {
+      int ex;
+      Q = (float)(2. * frexp(P, &ex));
+      k = (float)ldexp(127., min(1 - ex, 119));
+      Q = (float)ldexp((double)Q, min(1 - ex, 119) - (1 - ex));
+    }
+    inv = (R)1 / Q;
   }
   int8_t* cr = codes + row * c_sm;
   // (the row's tail: zeros up to a whole 128 bytes)
   const int padded = (D + kPad - 1) / kPad * kPad;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int at = (i * TPR + t) * VEC;
+    const int at = (i * TPR + t) * 8;
     if (at >= padded) continue;
-    int8_t c[VEC];
+    uint32_t c[8];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      // 127 p / P to the last bit: the quotient by the reciprocal, then its
-      // remainder's share
-      const double n = p[i * VEC + e] * 127., q0 = n * r, q = fma(fma(-q0, top, n), r, q0);
-      c[e] = fine ? (int8_t)(int)rint(q) : (int8_t)0;
+    for (int e = 0; e < 8; ++e) {
+      const R n = p[i * 8 + e] * k, q0 = n * inv;
+      const R q = __builtin_elementwise_fma(__builtin_elementwise_fma(-q0, Q, n), inv, q0) + kShift;
+      if constexpr (sizeof(R) == 4) c[e] = __builtin_bit_cast(uint32_t, q);
+      else c[e] = (uint32_t)__builtin_bit_cast(uint64_t, q);
     }
-    if constexpr (VEC == 8) {
-      uint2 v;
-      __builtin_memcpy(&v, c, 8);
-      *reinterpret_cast<uint2*>(cr + at) = v;
-    } else {
-      cr[at] = c[0];
+    uint2 v{0u, 0u};
+    if (fine) {
+      // the low bytes of four
+      const auto four = [](uint32_t a, uint32_t b, uint32_t cc, uint32_t d) {
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, cc, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                                     0x05040100u);
+      };
+      v = uint2{four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7])};
     }
+    *reinterpret_cast<uint2*>(cr + at) = v;
   }
 }
 
-template <typename T, bool NORM, bool RES, int VEC, int TPR, int IT>
+template <typename T, bool NORM, bool RES, int TPR, int IT>
 static int launch_codes(const T* x, int64_t x_sm, const T* res, int64_t r_sm, const T* w, int rows, int D, float eps,
                         T* sum_out, int64_t s_sm, int8_t* codes, int64_t c_sm, float* scales, hipStream_t st) {
   constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-  hipLaunchKernelGGL((codes_kernel<T, NORM, RES, VEC, TPR, IT>), dim3((unsigned)(((int64_t)rows + RPB - 1) / RPB)),
-                     dim3(NT), 0, st, x, x_sm, res, r_sm, w, rows, D, eps, sum_out, s_sm, codes, c_sm, scales);
+  hipLaunchKernelGGL((codes_kernel<T, NORM, RES, TPR, IT>), dim3((unsigned)(((int64_t)rows + RPB - 1) / RPB)), dim3(NT),
+                     0, st, x, x_sm, res, r_sm, w, rows, D, eps, sum_out, s_sm, codes, c_sm, scales);
   return check_launch("codes_kernel");
 }
 
 // threads and runs of a row of D elements (up to a multiple of 128)
 template <typename T, bool NORM, bool RES>
-static int run_codes(const void* x_, int64_t x_sm, const void* res_, int64_t r_sm, const void* w_, int rows, int D,
-                     float eps, void* sum_, int64_t s_sm, int8_t* codes, int64_t c_sm, float* scales, hipStream_t st) {
-  const T *x = (const T*)x_, *res = (const T*)res_, *w = (const T*)w_;
-  T* so = (T*)sum_;
+static int run_codes(const void* x, int64_t x_sm, const void* res, int64_t r_sm, const void* w, int rows, int D, float eps,
+                     void* sum, int64_t s_sm, int8_t* codes, int64_t c_sm, float* scales, hipStream_t st) {
   const int P = (D + kPad - 1) / kPad * kPad;
-  constexpr uintptr_t run = 8 * sizeof(T);
-  bool vec = D % 8 == 0 && x_sm % 8 == 0 && (uintptr_t)x % run == 0;
-  if (NORM) vec = vec && (uintptr_t)w % run == 0;
-  if (RES) vec = vec && r_sm % 8 == 0 && s_sm % 8 == 0 && (uintptr_t)res % run == 0 && (uintptr_t)so % run == 0;
-#define CODES(V, TPR, IT) \
-  return launch_codes<T, NORM, RES, V, TPR, IT>(x, x_sm, res, r_sm, w, rows, D, eps, so, s_sm, codes, c_sm, scales, st)
-  if (vec) {
-    if (P <= 1024) CODES(8, 64, 2);
-    if (P <= 2048) CODES(8, 256, 1);
-    if (P <= 4096) CODES(8, 256, 2);
-    if (P <= 8192) CODES(8, 512, 2);
-    CODES(8, 1024, 4);
-  }
-  if (P <= 1024) CODES(1, 64, 16);
-  if (P <= 8192) CODES(1, 512, 16);
-  CODES(1, 1024, 32);
+#define CODES(TPR, IT)                                                                                                   \
+  return launch_codes<T, NORM, RES, TPR, IT>((const T*)x, x_sm, (const T*)res, r_sm, (const T*)w, rows, D, eps, (T*)sum, \
+                                             s_sm, codes, c_sm, scales, st)
+  if (P <= 512) CODES(64, 1);
+  if (P <= 1024) CODES(64, 2);
+  if (P <= 2048) CODES(256, 1);
+  if (P <= 4096) CODES(256, 2);
+  if (P <= 8192) CODES(512, 2);
+  if (P <= 16384) CODES(1024, 2);
+  CODES(1024, 4);
 #undef CODES
 }
 
-// values of codes: out = code * scale, one rounding
-template <typename T>
+// values of codes: out = code * scale, one rounding to T.  TPR threads a row
+// and workgroup, 8 codes each; out rows of any element address.
+template <typename T, int TPR>
 __global__ __launch_bounds__(256) void values_kernel(const int8_t* __restrict__ codes, int64_t c_sm,
-                                                     const float* __restrict__ scales, int D, T* __restrict__ out,
-                                                     int64_t o_sm) {
-  const int64_t row = blockIdx.x;
+                                                     const float* __restrict__ scales, int rows, int D,
+                                                     T* __restrict__ out, int64_t o_sm) {
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int at = (blockIdx.y * TPR + threadIdx.x % TPR) * 8;
+  if (row >= rows || at >= D) return;
+  int8_t c[8];
+  const uint2 raw = *reinterpret_cast<const uint2*>(codes + row * c_sm + at);
+  __builtin_memcpy(c, &raw, 8);
   const float sc = scales[row];
-  for (int i = threadIdx.x; i < D; i += 256) out[row * o_sm + i] = Elt<T>::st((float)codes[row * c_sm + i] * sc);
+  T* o = out + row * o_sm + at;
+  Run8<T> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v.v[e] = Elt<T>::st((float)c[e] * sc);
+  run_st(o, D - at, v);
+}
+template <typename T>
+static int run_values(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, void* out, int64_t o_sm,
+                      hipStream_t st) {
+  // (a row of up to 512 elements leaves most of 256 threads idle)
+  if (D <= 512)
+    hipLaunchKernelGGL((values_kernel<T, 64>), dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(256), 0, st, codes, c_sm,
+                       scales, rows, D, (T*)out, o_sm);
+  else
+    hipLaunchKernelGGL((values_kernel<T, 256>), dim3((unsigned)rows, (unsigned)((D + 2047) / 2048)), dim3(256), 0, st,
+                       codes, c_sm, scales, rows, D, (T*)out, o_sm);
+  return check_launch("values_kernel");
 }
 
 // ------------------------------------------------------------ product
@@ -304,8 +374,8 @@ __device__ __forceinline__ void each(F&& f) {
 // (its first operands are read ahead, so that no product waits for LDS after
 // a barrier), step k + 2 is on its way and step k + 3 is asked for: one
 // barrier a step.  A stage holds a row's four 16-byte pieces in the order
-// slot = piece ^ (row / 2) % 4, by which eight lanes that read one piece of
-// eight rows touch every bank once.
+// slot = piece ^ (row / 4) % 4, by which the 16 lanes that LDS serves at once
+// (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
 template <int S>
 struct TileLds {
   static constexpr int kRows = 128 * S;       // features, then tokens
@@ -332,15 +402,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
   const int8_t* src[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int r = (4 * i + wv) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 1) & 3);
+    const int r = (4 * i + wv) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
     src[i] = r < BF ? W.p + (int64_t)min(f0 + r, W.rows - 1) * W.sm + 16 * piece
                     : X.p + (int64_t)min(m0 + r - BF, X.rows - 1) * X.sm + 16 * piece;
   }
   const int steps = K / 64;
+  auto load1 = [&](int k, int i) {
+    tile_load16(src[i] + (int64_t)k * 64, smem + (k & 3) * L::kStage + wv * 1024 + i * 4096);
+  };
   auto load = [&](int k) {
-    char* st = smem + (k & 3) * L::kStage + wv * 1024;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) tile_load16(src[i] + (int64_t)k * 64, st + i * 4096);
+    for (int i = 0; i < NL; ++i) load1(k, i);
   };
   i32x16 acc[S][S];
 #pragma unroll
@@ -351,22 +423,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   // operands of half h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
-  const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 1) & 3)) << 4);
+  const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 2) & 3)) << 4);
   i32x4 op[2][2 * S];
   auto read = [&](auto c, i32x4 (&o)[2 * S], uint32_t a) {  // operand c: S of features, S of tokens
     constexpr int i = decltype(c)::value;
     o[i] = i < S ? tile_read<i * 2048>(a + wf * (S * 2048)) : tile_read<BF * 64 + (i - S) * 2048>(a + wm * (S * 2048));
   };
-  // products of one half, and meanwhile the reads of the next
-  auto half = [&](i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a) {
+  // Products of half h of a step, and beside them the reads of the next half
+  // (early, so that they land before its first product) and half of step
+  // k + 3's loads (late and apart: asked for all at once before the products,
+  // they hold the wave up for as long as half of the products take).
+  auto half = [&](auto hc, auto more, i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a, int k) {
+    constexpr int h = decltype(hc)::value;
     each<S * S>([&](auto c) {
       constexpr int q = decltype(c)::value, i = q / S, j = q % S;
-      // (2 S reads beside the first half of the products)
-      constexpr int per = S == 1 ? 2 : S == 2 ? 2 : 1;
-      each<per>([&](auto d) {
-        constexpr int k = q * per + decltype(d)::value;
-        if constexpr (k < 2 * S) read(std::integral_constant<int, k>{}, next, a);
+      constexpr int reads = S == 4 ? 1 : 2;                               // a product
+      constexpr int first = S * S / 2, gap = S == 4 ? 2 : 1;              // loads beside products first, first + gap ..
+      each<reads>([&](auto d) {
+        constexpr int o = q * reads + decltype(d)::value;
+        if constexpr (o < 2 * S) read(std::integral_constant<int, o>{}, next, a);
       });
+      if constexpr (decltype(more)::value && q >= first && (q - first) % gap == 0)
+        load1(k + 3, h * (NL / 2) + (q - first) / gap);
       acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[S + j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -383,20 +461,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
   __builtin_amdgcn_s_barrier();
   each<2 * S>([&](auto c) { read(c, op[0], at); });
   tile_landed(op[0]);
-  for (int k = 0; k < steps; ++k) {
-    // here: step k + 1 has landed for every wave, all have done with k - 1
-    if (k + 3 < steps) load(k + 3);
-    __builtin_amdgcn_sched_barrier(0);
+  // at the start of step k: k + 1 has landed for every wave, all are done with k - 1
+  auto step = [&](auto more, int k) {
     const uint32_t here = at + (k & 3) * L::kStage;
     // (past the last step: its own operands again)
     const uint32_t then = at + (min(k + 1, steps - 1) & 3) * L::kStage;
-    half(op[0], op[1], here ^ 32);
-    half(op[1], op[0], then);
-    if (k + 3 < steps) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);  // step k + 2 has landed
-    else __builtin_amdgcn_s_waitcnt(0x0f70);
+    half(std::integral_constant<int, 0>{}, more, op[0], op[1], here ^ 32, k);
+    half(std::integral_constant<int, 1>{}, more, op[1], op[0], then, k);
+    // step k + 2 has landed
+    __builtin_amdgcn_s_waitcnt(decltype(more)::value ? ((NL & 15) | 0x0f70) : 0x0f70);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-  }
+  };
+  int k = 0;
+  for (; k + 3 < steps; ++k) step(std::true_type{}, k);
+  for (; k < steps; ++k) step(std::false_type{}, k);
   // Values pass through LDS (a wave's own part) from four features of 32
   // tokens a lane to runs of a token's features, 32 tokens at a time; the
   // features' scales and biases lie there too
@@ -545,14 +624,12 @@ extern "C" int coda_dequantize_rows(int dtype, const int8_t* codes, int64_t c_sm
   CODA_REQUIRE(rows >= 0 && D > 0, "%s: bad sizes rows=%d D=%d", who, rows, D);
   if (rows == 0) return CODA_OK;
   CODA_REQUIRE(codes && scales && out, "%s: null pointer", who);
+  CODA_REQUIRE((uintptr_t)codes % 16 == 0 && c_sm % 16 == 0 && c_sm >= (D + kPad - 1) / kPad * kPad && D <= kMaxK,
+               "%s: rows of codes must lie at 16-byte addresses and hold D=%d up to a multiple of %d", who, D, kPad);
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T)                                                                                                      \
-  hipLaunchKernelGGL((values_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, codes, c_sm, scales, D, (T*)out, o_sm)
-  if (dtype == CODA_F32) RUN(float);
-  else if (dtype == CODA_BF16) RUN(bf16_t);
-  else RUN(f16_t);
+#define RUN(T) run_values<T>(codes, c_sm, scales, rows, D, out, o_sm, st)
+  return dtype == CODA_F32 ? RUN(float) : dtype == CODA_BF16 ? RUN(bf16_t) : RUN(f16_t);
 #undef RUN
-  return check_launch("values_kernel");
 }
 
 extern "C" int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const float* x_scales, int M, const int8_t* w,
