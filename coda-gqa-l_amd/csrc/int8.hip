@@ -267,18 +267,19 @@ struct Int8Mat {
   int rows;
 };
 
-// four features of a token, rounded to T
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T v[4];
+// N features of a token, rounded to T
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Feats {
+  T v[N];
 };
 
-// Where the values of a product go: bias1(f) what is added to feature f;
-// lane(f) what a lane that writes features f .. f + 3 (a multiple of 4) of
-// several tokens needs to know once; put() writes them for token m.
+// Where the values of a product go: bias1(f) is added to feature f; lane(f) is
+// what a lane that writes features f .. f + N - 1 of several tokens needs to
+// know once, put() writes them for token m (N = 4, or kRun; f a multiple).
 template <typename T>
 struct LinearSink {
   typedef T Out;
+  static constexpr int kRun = 16 / sizeof(T);
   T* out;
   const T* bias;  // or null
   int64_t o_sm;
@@ -289,17 +290,17 @@ struct LinearSink {
   };
   __device__ __forceinline__ float bias1(int f) const { return bias ? Elt<T>::ld(bias[f]) : 0.f; }
   __device__ __forceinline__ Lane lane(int f) const { return Lane{out + f, n_feat - f}; }
-  __device__ __forceinline__ void put(const Lane& l, int m, const Four<T>& v) const {
+  template <int N>
+  __device__ __forceinline__ void put(const Lane& l, int m, const Feats<T, N>& v) const {
     // (rows of any element address)
-    typedef uint16_t u16x4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(4)));
-    typedef typename std::conditional<sizeof(T) == 2, u16x4, u32x4>::type V;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(2)));
+    typedef typename std::conditional<sizeof(v) == 8, u32x2, pu32x4u>::type V;
     T* row = l.p + (int64_t)m * o_sm;
-    if (l.n >= 4) {
+    if (l.n >= N) {
       *reinterpret_cast<V*>(row) = __builtin_bit_cast(V, v);
     } else {
 #pragma unroll
-      for (int e = 0; e < 3; ++e)
+      for (int e = 0; e < N - 1; ++e)
         if (e < l.n) row[e] = v.v[e];
     }
   }
@@ -312,6 +313,7 @@ struct NoBias {
 template <typename T>
 struct FrontSink {
   typedef T Out;
+  static constexpr int kRun = 4;
   FrontEpilogue<T, true> epi;
   int n_feat;
   struct Lane {
@@ -319,17 +321,19 @@ struct FrontSink {
   };
   __device__ __forceinline__ float bias1(int f) const { return epi.d.bias[f]; }
   __device__ __forceinline__ Lane lane(int f) const { return Lane{f}; }
-  __device__ __forceinline__ void put(const Lane& l, int m, const Four<T>& v) const {
+  __device__ __forceinline__ void put(const Lane& l, int m, const Feats<T, 4>& v) const {
     using E = Elt<T>;
     epi(NoBias{}, l.f, m, pf32x4{E::ld(v.v[0]), E::ld(v.v[1]), E::ld(v.v[2]), E::ld(v.v[3])});
   }
 };
 
+// three roundings to fp32 (the sum, times the token's scale, times the
+// channel's plus bias) and the one to T
 template <typename T>
-__device__ __forceinline__ Four<T> int8_value(const i32x4& a, float sx, const pf32x4& sw, const pf32x4& bias) {
-  Four<T> v;
+__device__ __forceinline__ Feats<T, 4> int8_value(const i32x4& a, float sx, const pf32x4& sw, const pf32x4& bias) {
+  Feats<T, 4> v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v.v[e] = Elt<T>::st((float)a[e] * sx * sw[e] + bias[e]);
+  for (int e = 0; e < 4; ++e) v.v[e] = Elt<T>::st(fmaf((float)a[e] * sx, sw[e], bias[e]));
   return v;
 }
 
@@ -368,6 +372,15 @@ __device__ __forceinline__ void each(F&& f) {
   each_impl(f, std::make_integer_sequence<int, N>{});
 }
 
+// An accumulator out of its AGPR, here and not earlier: the compiler would
+// move all 256 at once, over registers that the loop then lacks.  (The
+// caller is a barrier behind the last product: no hazard is left.)
+__device__ __forceinline__ int32_t acc_read(int32_t a) {
+  int32_t v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
+}
+
 // 4 waves (2 x 2) make 64 S features x 64 S tokens, a wave 32 S x 32 S in
 // S x S accumulators of 32 x 32.  K passes through LDS in steps of 64 bytes,
 // four stages: while the products of step k run, step k + 1 lies in LDS
@@ -376,51 +389,78 @@ __device__ __forceinline__ void each(F&& f) {
 // barrier a step.  A stage holds a row's four 16-byte pieces in the order
 // slot = piece ^ (row / 4) % 4, by which the 16 lanes that LDS serves at once
 // (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
-template <int S>
+// A workgroup of the largest tile (S = 4: one a CU) goes from tile to tile;
+// the stages run on over the border, so that the next tile's first steps are
+// in LDS when this one's values have been written, and the writes are on
+// their way while its products run.
+template <int S, typename T>
 struct TileLds {
   static constexpr int kRows = 128 * S;       // features, then tokens
   static constexpr int kStage = kRows * 64;   // bytes
-  static constexpr int kStages = 4;
-  static constexpr size_t kBytes = (size_t)kStages * kStage;
+  static constexpr bool kWalk = S == 4;
+  // a wave's values on their way out: 32 tokens x kFeats features
+  static constexpr int kFeats = kWalk ? 128 / (int)sizeof(T) : 32 * S;
+  static constexpr int kRow = kFeats * sizeof(T) + 16;
+  static constexpr int kScales = 3 * 64 * S * sizeof(float);  // features' scales, biases, tokens' scales
+  static constexpr int kOut = kWalk ? 4 * kStage : 0;         // (smaller tiles: over the stages)
+  static constexpr size_t kEnd = kOut + kScales + 4 * 32 * kRow;
+  static constexpr size_t kBytes = kEnd > 4 * kStage ? kEnd : 4 * kStage;
 };
 template <int S, typename Sink>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 : 2))) void int8_tile(
     const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
   typedef typename Sink::Out T;
-  typedef TileLds<S> L;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef TileLds<S, T> L;
+  extern __shared__ __attribute__((aligned(128))) char smem[];
   constexpr int BF = 64 * S, BM = 64 * S, NL = L::kRows / 64;  // loads a thread and step
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
   // in groups of 4 token tiles, so that what it has at a time shares rows in
-  // its L2.
+  // its L2; its workgroups take them in turn.
   const int n = ntf * ntm, xcd = blockIdx.x & 7, base = n >> 3, rem = n & 7;
-  const int t = xcd * base + min(xcd, rem) + (int)(blockIdx.x >> 3);
-  const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
-  const int f0 = in / gm * BF, m0 = (4 * group + in % gm) * BM;
-  // this lane's pieces: rows of a load are 16, four pieces each
-  const int8_t* src[NL];
-#pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int r = (4 * i + wv) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
-    src[i] = r < BF ? W.p + (int64_t)min(f0 + r, W.rows - 1) * W.sm + 16 * piece
-                    : X.p + (int64_t)min(m0 + r - BF, X.rows - 1) * X.sm + 16 * piece;
-  }
-  const int steps = K / 64;
-  auto load1 = [&](int k, int i) {
-    tile_load16(src[i] + (int64_t)k * 64, smem + (k & 3) * L::kStage + wv * 1024 + i * 4096);
+  const int t0 = xcd * base + min(xcd, rem), end = t0 + base + (xcd < rem ? 1 : 0);
+  const int turn = ((int)gridDim.x - xcd + 7) >> 3;
+  struct At {
+    int f, m;
   };
-  auto load = [&](int k) {
+  auto place = [&](int t) {
+    const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
+    return At{in / gm * BF, (4 * group + in % gm) * BM};
+  };
+  // this lane's pieces, as offsets from a tile's first rows: a load is 16 rows
+  // of four pieces, the first half of them features
+  uint32_t src[NL];
+  const int8_t *wsrc, *xsrc;
+  auto aim = [&](const At& a) {
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (nothing of this is worth a register between tiles)
 #pragma unroll
-    for (int i = 0; i < NL; ++i) load1(k, i);
+    for (int i = 0; i < NL; ++i) {
+      const int r = (4 * (i % S) + wv) * 16 + (l >> 2), piece = (l & 3) ^ ((r >> 2) & 3);
+      src[i] = 16 * piece + (i < S ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
+                                   : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
+    }
+    wsrc = W.p + a.f * W.sm;
+    xsrc = X.p + a.m * X.sm;
+  };
+  // the loads: tile lt's step lk into stage ls; on to the next tile at its end
+  const int steps = K / 64;
+  int tile = t0 + (int)(blockIdx.x >> 3), lt = tile, lk = 0, ls = 0;
+  auto load1 = [&](auto c) {
+    constexpr int i = decltype(c)::value;
+    tile_load16((i < S ? wsrc : xsrc) + src[i], smem + (ls & 3) * L::kStage + wv * 1024 + i * 4096);
+  };
+  auto loaded = [&]() {
+    ++ls;
+    wsrc += 64;
+    xsrc += 64;
+    if (++lk == steps) {
+      lk = 0;
+      lt = L::kWalk ? lt + turn : end;
+      if (lt < end) aim(place(lt));
+    }
   };
   i32x16 acc[S][S];
-#pragma unroll
-  for (int i = 0; i < S; ++i)
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   // operands of half h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
   const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 2) & 3)) << 4);
@@ -430,98 +470,140 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
     o[i] = i < S ? tile_read<i * 2048>(a + wf * (S * 2048)) : tile_read<BF * 64 + (i - S) * 2048>(a + wm * (S * 2048));
   };
   // Products of half h of a step, and beside them the reads of the next half
-  // (early, so that they land before its first product) and half of step
-  // k + 3's loads (late and apart: asked for all at once before the products,
+  // (early, so that they land before its first product) and half of a later
+  // step's loads (late and apart: asked for all at once before the products,
   // they hold the wave up for as long as half of the products take).
-  auto half = [&](auto hc, auto more, i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a, int k) {
+  auto half = [&](auto hc, auto more, i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a) {
     constexpr int h = decltype(hc)::value;
     each<S * S>([&](auto c) {
       constexpr int q = decltype(c)::value, i = q / S, j = q % S;
-      constexpr int reads = S == 4 ? 1 : 2;                               // a product
-      constexpr int first = S * S / 2, gap = S == 4 ? 2 : 1;              // loads beside products first, first + gap ..
+      constexpr int reads = S == 4 ? 1 : 2;                   // a product
+      constexpr int first = S * S / 2, gap = S == 4 ? 2 : 1;  // loads beside products first, first + gap ..
       each<reads>([&](auto d) {
         constexpr int o = q * reads + decltype(d)::value;
         if constexpr (o < 2 * S) read(std::integral_constant<int, o>{}, next, a);
       });
       if constexpr (decltype(more)::value && q >= first && (q - first) % gap == 0)
-        load1(k + 3, h * (NL / 2) + (q - first) / gap);
+        load1(std::integral_constant<int, h * (NL / 2) + (q - first) / gap>{});
       acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[S + j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
     tile_landed(next);
   };
-  // (K is a multiple of 128: two steps at least)
-  load(0);
-  load(1);
-  if (steps > 2) load(2);
+  // At the start of step g: g + 1 has landed for every wave, all are done with
+  // g - 1.  more: the loads are three steps ahead still; wait: for g + 2, the
+  // last but one that was asked for (or, without more, the last).
+  int g = 0;
+  auto step = [&](auto more, auto wait) {
+    const uint32_t here = at + (g & 3) * L::kStage, then = at + ((g + 1) & 3) * L::kStage;
+    half(std::integral_constant<int, 0>{}, more, op[0], op[1], here ^ 32);
+    half(std::integral_constant<int, 1>{}, more, op[1], op[0], then);
+    if constexpr (decltype(more)::value) loaded();
+    if constexpr (decltype(wait)::value && decltype(more)::value) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
+    else if constexpr (decltype(wait)::value) __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    ++g;
+  };
+  aim(place(tile));
+  for (int s = 0; s < 3 && lt < end; ++s) {
+    each<NL>([&](auto c) { load1(c); });
+    loaded();
+  }
   __builtin_amdgcn_sched_barrier(0);
-  // steps 0 and 1 have landed
-  if (steps > 2) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
+  // steps 0 and 1 have landed (K is a multiple of 128: there are two)
+  if (ls == 3) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
   else __builtin_amdgcn_s_waitcnt(0x0f70);
   __builtin_amdgcn_s_barrier();
   each<2 * S>([&](auto c) { read(c, op[0], at); });
   tile_landed(op[0]);
-  // at the start of step k: k + 1 has landed for every wave, all are done with k - 1
-  auto step = [&](auto more, int k) {
-    const uint32_t here = at + (k & 3) * L::kStage;
-    // (past the last step: its own operands again)
-    const uint32_t then = at + (min(k + 1, steps - 1) & 3) * L::kStage;
-    half(std::integral_constant<int, 0>{}, more, op[0], op[1], here ^ 32, k);
-    half(std::integral_constant<int, 1>{}, more, op[1], op[0], then, k);
-    // step k + 2 has landed
-    __builtin_amdgcn_s_waitcnt(decltype(more)::value ? ((NL & 15) | 0x0f70) : 0x0f70);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  int k = 0;
-  for (; k + 3 < steps; ++k) step(std::true_type{}, k);
-  for (; k < steps; ++k) step(std::false_type{}, k);
-  // Values pass through LDS (a wave's own part) from four features of 32
-  // tokens a lane to runs of a token's features, 32 tokens at a time; the
-  // features' scales and biases lie there too
-  constexpr int ROW = 32 * S * sizeof(T) + 16, QR = 8 * S;  // bytes of a row, fours of features in it
-  float* fs = reinterpret_cast<float*>(smem);
-  if (threadIdx.x < BF) {
-    const int f = min(f0 + (int)threadIdx.x, W.rows - 1);
-    fs[threadIdx.x] = W.scales[f];
-    fs[BF + threadIdx.x] = sink.bias1(f);
-  }
-  __syncthreads();
-  char* mine = smem + 2 * BF * sizeof(float) + wv * 32 * ROW;
-  const int fw = f0 + 32 * S * wf, mw = m0 + 32 * S * wm, q = lane % QR, fq = fw + 4 * q;
-  const typename Sink::Lane to = sink.lane(min(fq, W.rows - 1));
-  const char* own = smem + (32 * S * wf + 4 * (lane >> 5)) * sizeof(float);
-  each<S>([&](auto jc) {
-    constexpr int j = decltype(jc)::value;
-    const float sx = X.scales[min(mw + 32 * j + r32, X.rows - 1)];
-    each<4 * S>([&](auto gc) {
-      constexpr int i = decltype(gc)::value / 4, g = decltype(gc)::value % 4, fl = 32 * i + 8 * g;
-      const pf32x4 sw = *reinterpret_cast<const pf32x4*>(own + fl * sizeof(float));
-      const pf32x4 bias = *reinterpret_cast<const pf32x4*>(own + (BF + fl) * sizeof(float));
-      const i32x4 a{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-      *reinterpret_cast<Four<T>*>(mine + r32 * ROW + (fl + 4 * (lane >> 5)) * sizeof(T)) = int8_value<T>(a, sx, sw, bias);
-    });
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 4
-    for (int r = 0; r < 32; r += 64 / QR) {
-      const int row = r + lane / QR, m = mw + 32 * j + row;
-      const Four<T> v = *reinterpret_cast<const Four<T>*>(mine + row * ROW + q * 4 * sizeof(T));
-      if (m < X.rows && fq < W.rows) sink.put(to, m, v);
+  for (;;) {
+    const At a = place(tile);
+    float scale[3] = {0.f, 0.f, 0.f};
+    const int own = (int)threadIdx.x;
+    if (own < BF) {
+      const int f = min(a.f + own, W.rows - 1);
+      scale[0] = W.scales[f];
+      scale[1] = sink.bias1(f);
+      scale[2] = X.scales[min(a.m + own, X.rows - 1)];
     }
-    __builtin_amdgcn_wave_barrier();
-  });
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+    int k = 0;
+    // (a later tile: its second step has landed before the values were written)
+    if (g > 0 && lt < end) {
+      step(std::true_type{}, std::false_type{});
+      ++k;
+    }
+    for (; k < steps && lt < end; ++k) step(std::true_type{}, std::true_type{});
+    for (; k < steps; ++k) step(std::false_type{}, std::true_type{});
+    // Values pass through LDS (a wave's own part) from four features of 32
+    // tokens a lane to runs of a token's features
+    int le = lane;
+    asm volatile("" : "+v"(le));  // (nor are these addresses)
+    float* fs = reinterpret_cast<float*>(smem + L::kOut);
+    if (own < BF) {
+      fs[own] = scale[0];
+      fs[BF + own] = scale[1];
+      fs[2 * BF + own] = scale[2];
+    }
+    // every load so far has landed: the writes below do not hold up the
+    // next steps' waits
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    constexpr int N = Sink::kRun, PR = L::kFeats / N, NF = L::kFeats / 32;  // runs of a row, blocks of 32 features
+    char* mine = smem + L::kOut + L::kScales + wv * 32 * L::kRow;
+    const int fw = 32 * S * wf, mw = 32 * S * wm, fq = le % PR * N;
+    const float* fl = fs + fw + 4 * (le >> 5);
+    each<S>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      const float sx = fs[2 * BF + mw + 32 * j + (le & 31)];
+      each<S / NF>([&](auto pc) {
+        constexpr int part = decltype(pc)::value;
+        each<4 * NF>([&](auto gc) {
+          constexpr int q = decltype(gc)::value, i = part * NF + q / 4, r = q % 4, f = 32 * i + 8 * r;
+          const pf32x4 sw = *reinterpret_cast<const pf32x4*>(fl + f);
+          const pf32x4 bias = *reinterpret_cast<const pf32x4*>(fl + BF + f);
+          i32x4 v;
+          each<4>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            v[e] = L::kWalk ? acc_read(acc[i][j][4 * r + e]) : acc[i][j][4 * r + e];
+          });
+          *reinterpret_cast<Feats<T, 4>*>(mine + (le & 31) * L::kRow + (32 * (q / 4) + 8 * r + 4 * (le >> 5)) * sizeof(T)) =
+              int8_value<T>(v, sx, sw, bias);
+        });
+        __builtin_amdgcn_wave_barrier();
+        const int f = a.f + fw + part * L::kFeats + fq;
+        const typename Sink::Lane to = sink.lane(min(f, W.rows - 1));
+#pragma unroll
+        for (int r = 0; r < 32; r += 64 / PR) {
+          const int row = r + le / PR, m = a.m + mw + 32 * j + row;
+          const Feats<T, N> v = *reinterpret_cast<const Feats<T, N>*>(mine + row * L::kRow + fq * sizeof(T));
+          if (m < X.rows && f < W.rows) sink.put(to, m, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+      });
+    });
+    if (!L::kWalk) break;
+    tile += turn;
+    if (tile >= end) break;
+  }
 }
 
 template <int S, typename Sink>
 static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  typedef TileLds<S> L;
+  typedef TileLds<S, typename Sink::Out> L;
   const int64_t ntf = ((int64_t)W.rows + 64 * S - 1) / (64 * S), ntm = ((int64_t)X.rows + 64 * S - 1) / (64 * S);
-  if (ntf * ntm > INT_MAX) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)(ntf * ntm));
-  constexpr size_t values = (size_t)2 * 64 * S * 4 + 4 * 32 * (32 * S * sizeof(typename Sink::Out) + 16);
-  constexpr size_t lds = values > L::kBytes ? values : L::kBytes;
-  const int rc = lds_limit<int8_tile<S, Sink>>(lds, who);
+  const int64_t n = ntf * ntm;
+  if (n > INT_MAX / 8) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
+  const int rc = lds_limit<int8_tile<S, Sink>>(L::kBytes, who);
   if (rc) return rc;
-  hipLaunchKernelGGL((int8_tile<S, Sink>), dim3((unsigned)(ntf * ntm)), dim3(256), lds, st, X, W, K, (int)ntf, (int)ntm,
+  const int64_t grid = L::kWalk && n > device_cus() ? device_cus() : n;
+  hipLaunchKernelGGL((int8_tile<S, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
                      sink);
   return check_launch("int8_tile");
 }
