@@ -90,6 +90,12 @@ class _CoDAAdapter(nn.Module):
             y, self._state = self.coda.prefill_chunked(x, self._state, block_size=self.block_size)
         return y
 
+    def use_int8_projections(self, on: bool = True) -> "_CoDAAdapter":
+        """The layer's projections in 8 bits (Int8Mixin.use_int8_projections);
+        the adapter then takes the Int8Rows of rms_norm_int8 as well."""
+        self.coda.use_int8_projections(on)
+        return self
+
     # ------------------------------------------------------------ state
     def init_inference_state(self, batch_size: int, device: torch.device,
                              dtype: torch.dtype) -> CoDAGQALandmarkStatePerf2:

@@ -29,6 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import _hip, ops
+from .int8 import Int8Mixin, Int8Rows, _flat
 from .memory_banks import METRIC_KEYS, DeviceMetrics, MemoryBankMixin
 from .primitives import HeadwiseRMSNorm, RotaryEmbedding, apply_rope
 from .rows import RowsMixin, _aligned, _capturing, _version
@@ -37,7 +38,7 @@ from .state import CoDAGQALandmarkStatePerf2
 __all__ = ["CoDAGQALandmarkPerf2", "CoDAGQALandmarkStatePerf2"]
 
 
-class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
+class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
     def __init__(
         self,
         *,
@@ -296,6 +297,9 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         kernel in place, q / k / v / lambda as strided views of its output)
         faulted the GPU once in a full-size prefill, with no cause shown; it
         was removed, and prefill keeps the torch linears."""
+        if self._int8_on(x):
+            q, k, v, g, lam, cos, sin = self._front_int8(x, p0)
+            return q, k, v, torch.ones(x.shape[:2], device=x.device) if g is None else g, lam, cos, sin
         B, L, D = x.shape
         H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
         Fq, Fk = H * Dh, Hkv * Dh
@@ -395,6 +399,9 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         assert L == 1
         self._check_state(state)
         qp = int(state.pos if query_pos is None else query_pos)
+        if self._int8_on(x):
+            q, _, _, _, lam, cos, sin = self._front(x, qp)
+            return self._out_proj(self.decode_attend_core(q, lam, state, cos, sin).view(B, 1, -1))
         cos, sin = self.rope(seq_len=1, offset=qp, device=x.device, dtype=x.dtype)
         heads = self.decode_attend_core(self._project_q(x), self._lambda(x), state, cos, sin)
         return self.o_proj(heads.view(B, 1, self.num_heads * self.head_dim))
@@ -410,6 +417,10 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         q_pos = int(state.pos)
 
         def write():
+            if self._int8_on(x):
+                _, k_new, v_new, g_new, _, _, _ = self._front(x, q_pos)
+                self._write_one(state, k_new=k_new, v_new=v_new, g_new=g_new)
+                return
             k_raw, v_new = self._project_kv_raw(x)
             cosk, sink = self.rope(seq_len=1, offset=q_pos, device=x.device, dtype=x.dtype)
             k_new = apply_rope(k_raw, cosk, sink, interleaved=self.rope_interleaved)
@@ -420,6 +431,10 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
             if y is not None:
                 return y, state
             self._check_state(state)
+            if self._int8_on(x):
+                q, k_new, v_new, g, lam, cos, sin = self._front(x, q_pos)
+                heads = self.decode_step_core(q, k_new, v_new, g.reshape(B), lam, state, cos, sin, k_roped=True)
+                return self._out_proj(heads.view(B, 1, self.num_heads * self.head_dim)), state
             if self._fused_front_ok(x):
                 # one launch for q / k (roped) / v / lambda / gate
                 q, k_new, v_new, g, lam, cos, sin = self._front(x, q_pos, fused=True)
@@ -431,7 +446,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
             heads = self.decode_step_core(self._project_q(x), k_raw, v_new, self._write_gate(x).reshape(B),
                                           self._lambda(x), state, cos.contiguous(), sin.contiguous(), k_roped=False)
             return self.o_proj(heads.view(B, 1, self.num_heads * self.head_dim)), state
-        y = self.attend_step(x, state, query_pos=q_pos) if attend else torch.zeros_like(x)
+        y = self.attend_step(x, state, query_pos=q_pos) if attend else \
+            torch.zeros(x.shape, dtype=x.dtype, device=x.device)
         if write_cache:
             write()
         return y, state
@@ -440,7 +456,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         """A steady-state decode step (full ring, fixed bank sizes, no
         metrics or traces, decode-shaped input) from descriptors and
         buffers cached per state: per token the host sets the input and
-        RoPE-row pointers (packed weights) or the parameters' own addresses
+        RoPE-row pointers (packed weights, 8-bit projections) or the parameters' own addresses
         and the position (few-row inputs that those don't serve), makes two
         library calls (the projections, then coda_decode_step on their
         outputs) and o_proj.  Returns None when the general path must run
@@ -452,7 +468,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
                 self._expandable() or (self.Me == 0 and self.Ms == 0) or self._tracing() or \
                 _capturing():
             return None
-        packed, rows, angles = self._packed_front_ok(x), None, None
+        int8 = self._int8_on(x)
+        packed, rows, angles = int8 or self._packed_front_ok(x), None, None
         if not packed:
             rows = self._front_rows(x)
             angles = None if rows is None else self._angles_rows(x.device, int(st.pos), 1)
@@ -463,16 +480,19 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         vers = tuple(-1 if t is None else t._version for t in ts)
         pvers = self._param_key()
         B, stream = x.shape[0], _hip.stream_of(x)
-        if fp is None or fp["st"] is not st or fp["vers"] != vers or fp["pvers"] != pvers or fp["B"] != B or \
+        if fp is None or fp["int8"] != int8 or fp["st"] is not st or fp["vers"] != vers or fp["pvers"] != pvers or fp["B"] != B or \
                 fp["packed"] != packed or fp["dtype"] is not x.dtype or fp["stream"] != stream or \
                 fp["ptrs"] != tuple(-1 if t is None else t.data_ptr() for t in ts) or fp["dev"] != x.device:
-            fp = self._build_step_fast(x, st, ts, vers, pvers, packed)
+            fp = self._build_step_fast(x, st, ts, vers, pvers, packed, int8)
             if fp is None:
                 return None
-        x = _aligned(x)
         pos = int(st.pos)
         d, a = fp["proj"], fp["attn"]
-        d.x = x.data_ptr()
+        if int8:
+            scales = self._step_int8_tokens(fp, d, x, stream)
+        else:
+            x = _aligned(x)
+            d.x = x.data_ptr()
         cos_t, sin_t = fp["tab"]
         if packed:
             if pos >= cos_t.shape[0]:
@@ -481,7 +501,10 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
             row = fp["row_bytes"] * pos
             d.rope_cos = a.rope_cos = cos_t.data_ptr() + row
             d.rope_sin = a.rope_sin = sin_t.data_ptr() + row
-            _hip.check(fp["project"](fp["proj_ref"], stream))
+            if int8:
+                _hip.check(fp["project"](fp["proj_ref"], scales.data_ptr(), *fp["int8_args"], stream))
+            else:
+                _hip.check(fp["project"](fp["proj_ref"], stream))
         else:
             # (the launch writes the token's RoPE row to fp["tab"])
             if fp["rows"] != rows:
@@ -503,7 +526,21 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         fp["record_pos"] = pos + 1 if routed.value else -1
         # the general path's carried-record tag no longer matches this state
         self.__dict__["_route_tag"] = None
-        return self._out_rows(fp["heads_flat"], kept=True)
+        return self._out_proj(fp["heads_flat"]) if int8 else self._out_rows(fp["heads_flat"], kept=True)
+
+    def _step_int8_tokens(self, fp: dict, d, x, stream: int) -> torch.Tensor:
+        """The tokens of a cached step in 8 bits: their codes in d, their scales."""
+        if isinstance(x, Int8Rows):
+            codes, d.x_sm, scales = _flat(x)
+            d.x = codes.data_ptr()
+            fp["int8_rows"] = codes
+            return scales
+        codes, scales = fp["int8_tokens"]
+        x = _aligned(x)
+        d.x, d.x_sm = codes.data_ptr(), codes.shape[1]
+        _hip.check(_hip.lib().coda_quantize_rows(d.dtype, x.data_ptr(), x.shape[-1], x.shape[0], x.shape[-1], d.x, d.x_sm,
+                                                 scales.data_ptr(), stream))
+        return scales
 
     def _param_key(self) -> tuple:
         """Identity, storage and in-place version of every parameter of the
@@ -520,7 +557,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
                     out += (id(p), p.data_ptr(), p._version)
         return tuple(out)
 
-    def _build_step_fast(self, x, st, ts, vers, pvers, packed):
+    def _build_step_fast(self, x, st, ts, vers, pvers, packed, int8):
         """Descriptors and persistent buffers of _step_fast (see there)."""
         self.__dict__["_fast"] = None
         self._check_state(st)
@@ -548,7 +585,20 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
             cos_t, sin_t = torch.empty((2, 1, Dh // 2), dtype=dt, device=dev)
             row = slice(0, 1)
         d = self._proj_desc(x, B, 1, cos_t, sin_t)
-        if packed:
+        int8_args = int8_tokens = None
+        if int8:
+            if D != self.embed_dim:
+                return None
+            w, sw, b = self._int8_weights()[:3]
+            if w.device != dev:
+                raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
+            d.w, d.bias, int8_args = w.data_ptr(), b.data_ptr(), (sw.data_ptr(), w.stride(0), w.shape[1])
+            int8_tokens = (torch.empty((B, w.shape[1]), dtype=torch.int8, device=dev),
+                           torch.empty(B, dtype=torch.float32, device=dev))
+            w = (w, sw)
+            if not self._has_gate():
+                g.fill_(1.0)  # the launch leaves it alone
+        elif packed:
             w, b, d.w_layout = self._packed_weights(x)
             d.w, d.bias = w.data_ptr(), b.data_ptr()
         d.x_sm = D
@@ -573,7 +623,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         routed = ctypes.c_int(0)
 
         fp = {"st": st, "vers": vers, "pvers": pvers, "B": B, "dev": dev, "dtype": dt, "stream": _hip.stream_of(x),
-              "packed": packed, "rows": None, "step": L_.coda_decode_step,
+              "packed": packed, "int8": int8, "int8_args": int8_args, "int8_tokens": int8_tokens, "rows": None,
+              "step": L_.coda_decode_step,
               "ptrs": tuple(-1 if t is None else t.data_ptr() for t in ts),
               "tab": (cos_t, sin_t), "row_bytes": (Dh // 2) * cos_t.element_size(),
               "proj": d, "proj_ref": ctypes.byref(d), "attn": a, "attn_ref": ctypes.byref(a),
@@ -582,7 +633,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
               "k_ptr": k.data_ptr(), "v_ptr": v.data_ptr(), "k_sb": Fk, "k_sh": Dh, "g_ptr": g.data_ptr(),
               "ws_ptr": _hip.ptr(ws), "ws_bytes": nb.value, "routed": routed, "routed_ref": ctypes.byref(routed),
               "record_pos": routed_pos,
-              "project": L_.coda_project_rows if packed else L_.coda_project_params,
+              "project": L_.coda_project_int8 if int8 else L_.coda_project_rows if packed else L_.coda_project_params,
               "heads_flat": heads.view(B, 1, H * Dh)}
         self.__dict__["_fast"] = fp
         return fp
@@ -789,7 +840,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
         _hip.require_device(x_seq)
         B, L, _ = x_seq.shape
         if L == 0:
-            return (x_seq[:, :0, :].clone() if return_outputs else None), state
+            return (torch.empty(x_seq.shape, dtype=x_seq.dtype, device=x_seq.device) if return_outputs else None), state
         if block_size <= 0:
             raise ValueError("block_size must be positive")
         p0 = int(state.pos)
@@ -798,7 +849,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, RowsMixin, nn.Module):
                                   return_heads=return_outputs)
         if not return_outputs:
             return None, state
-        return self.o_proj(heads.view(B, L, self.num_heads * self.head_dim)), state
+        return self._out_proj(heads.view(B, L, self.num_heads * self.head_dim)), state
 
     # ------------------------------------------------------------ utility
     def cache_bytes(self, *, batch_size: int, dtype: torch.dtype) -> int:

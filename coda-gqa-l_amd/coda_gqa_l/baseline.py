@@ -17,11 +17,12 @@ import torch
 import torch.nn as nn
 
 from . import _hip, ops
+from .int8 import Int8Mixin
 from .primitives import HeadwiseRMSNorm, RotaryEmbedding, apply_rope
 from .rows import RowsMixin, _aligned
 
 
-class CoDAGQA(RowsMixin, nn.Module):
+class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
     def __init__(self, *, embed_dim: int, num_heads: int, num_kv_heads: int, rope_base: float = 10_000.0,
                  lambda_init_bias: float = -6.0, theta_init: float = math.pi / 2, eps: float = 1e-6,
                  head_norm_mode: str = "full", rope_interleaved: bool = True):
@@ -83,10 +84,20 @@ class CoDAGQA(RowsMixin, nn.Module):
         _hip.require_device(x)
         B, L, D = x.shape
         H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
-        if past_key_value is not None:
-            rows = self._decode_rows(x, past_key_value, is_causal)
+        int8 = self._int8_on(x)
+        if past_key_value is not None and self._decode_ok(x, past_key_value, is_causal):
+            if int8:
+                return self._decode_int8(x, *past_key_value)
+            rows = self._front_rows(x)
             if rows is not None:
                 return self._decode(x, rows, *past_key_value)
+        if int8:
+            offset = past_key_value[0].size(2) if past_key_value is not None else 0
+            q, k, v, _, lam, cos, sin = self._front_int8(x, offset)
+            if past_key_value is not None:
+                k, v = (torch.cat([p, n], dim=2) for p, n in zip(past_key_value, (k, v)))
+            heads = self.attention_core(q, k, v, lam, cos, sin, causal=2 if is_causal else 0)
+            return self._out_proj(heads.view(B, L, D)), (k, v)
         q = self.q_proj(x).view(B, L, H, Dh).permute(0, 2, 1, 3)
         k = self.k_proj(x).view(B, L, Hkv, Dh).permute(0, 2, 1, 3)
         v = self.v_proj(x).view(B, L, Hkv, Dh).permute(0, 2, 1, 3)
@@ -103,25 +114,23 @@ class CoDAGQA(RowsMixin, nn.Module):
         heads = self.attention_core(q, k, v, lam, cos, sin, causal=2 if is_causal else 0)
         return self.o_proj(heads.view(B, L, D)), (k, v)
 
-    def _decode_rows(self, x: torch.Tensor, past: Tuple[torch.Tensor, torch.Tensor], is_causal: bool):
-        """The parameters' addresses (_front_rows) where _decode serves this
-        call, else None: few new tokens on top of a past, no mask, bf16, at
+    def _decode_ok(self, x: torch.Tensor, past: Tuple[torch.Tensor, torch.Tensor], is_causal: bool) -> bool:
+        """Whether _decode serves this call as far as its attention goes: few
+        new tokens on top of a past, no mask, bf16, at
         most 8 / G tokens a sequence, row-aligned K / V of the layer's shape
         whose planes stay within the kernel's 31-bit offsets."""
         B, L, _ = x.shape
         k, v = past
         if is_causal or L == 0 or x.dtype != torch.bfloat16 or k.dtype != x.dtype or v.dtype != x.dtype or \
                 2 * L * (self.num_heads // self.num_kv_heads) > 16 or self.head_dim not in (32, 64, 128):
-            return None
+            return False
         shape = (B, self.num_kv_heads, k.shape[2] if k.dim() == 4 else 0, self.head_dim)
         st = k.stride()
-        if not (tuple(k.shape) == shape and tuple(v.shape) == shape and shape[2] > 0 and v.stride() == st and
+        return (tuple(k.shape) == shape and tuple(v.shape) == shape and shape[2] > 0 and v.stride() == st and
                 st[3] == 1 and not (st[0] % 8 or st[1] % 8 or st[2] % 8) and
                 0 <= st[2] and (shape[2] + L + 16) * max(st[2], self.head_dim) < 1 << 30 and
                 not (k.data_ptr() % 16 or v.data_ptr() % 16) and k.device == v.device == x.device and
-                not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad))):
-            return None
-        return self._front_rows(x)
+                not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)))
 
     def _decode(self, x: torch.Tensor, rows: tuple, k_past: torch.Tensor, v_past: torch.Tensor):
         """forward() on top of a past for a few new tokens: one launch for the
@@ -134,10 +143,6 @@ class CoDAGQA(RowsMixin, nn.Module):
         past, M, e, half = k_past.shape[2], B * L, x.element_size(), Dh // 2
         lib, stream, dev = _hip.lib(), _hip.stream_of(x), x.device
         xs = _aligned(x)
-        w = self.head_norm.weight.detach().to(x.dtype).contiguous() if self.head_norm_mode == "full" else None
-        a = _hip.AttnDesc()
-        a.dtype = _hip.dtype_code(x.dtype)
-        a.B, a.H, a.Hkv, a.Lq, a.Dh = B, H, Hkv, L, Dh
         # q | k | v | lambda | gate of the new tokens, RoPE cos | sin, theta
         # cos | sin in one buffer
         sizes = [M * D * e, M * Hkv * Dh * e, M * Hkv * Dh * e, M * H * e, M * 4, L * half * e, L * half * e,
@@ -146,8 +151,6 @@ class CoDAGQA(RowsMixin, nn.Module):
         for n in sizes:
             at.append(at[-1] + -(-n // 256) * 256)
         buf = torch.empty(at[-1], dtype=torch.uint8, device=dev)
-        heads = torch.empty((B, L, D), dtype=x.dtype, device=dev)
-        k, v = (torch.empty((B, Hkv, past + L, Dh), dtype=x.dtype, device=dev) for _ in range(2))
         q_p, k_p, v_p, l_p, g_p, rc_p, rs_p, tc_p, ts_p = (buf.data_ptr() + o for o in at[:-1])
         p = self._proj_params(rows)
         angles, th, keep = self._angles_rows(dev, past, L), self.theta, ()
@@ -161,7 +164,7 @@ class CoDAGQA(RowsMixin, nn.Module):
                 th.is_contiguous():
             p.theta, p.theta_dtype, p.theta_cos, p.theta_sin = th.data_ptr(), _hip.dtype_code(th.dtype), tc_p, ts_p
         else:
-            tt = tuple(f(th).to(dtype=x.dtype).contiguous() for f in (torch.cos, torch.sin))
+            tt = self._theta_pair(x.dtype)
             tc_p, ts_p = (t.data_ptr() for t in tt)
             keep += tt
         d = self._proj_desc(x, M, L)
@@ -170,6 +173,34 @@ class CoDAGQA(RowsMixin, nn.Module):
         d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q_p, D, k_p, Hkv * Dh, v_p, Hkv * Dh
         d.lam, d.lam_sm, d.g = l_p, H, g_p
         _hip.check(lib.coda_project_params(d, p, stream))
+        heads, kv = self._append(x, (q_p, k_p, v_p, l_p, rc_p, rs_p, tc_p, ts_p), k_past, v_past)
+        return self._out_rows(heads), kv
+
+    def _decode_int8(self, x, k_past: torch.Tensor, v_past: torch.Tensor):
+        """_decode with 8-bit projections."""
+        q, k, v, _, lam, cos, sin = self._front_int8(x, k_past.shape[2])
+        keep = (q, k, v, lam, cos, sin, *self._theta_pair(x.dtype))
+        heads, kv = self._append(x, tuple(t.data_ptr() for t in keep), k_past, v_past)
+        return self._out_proj(heads), kv
+
+    def _theta_pair(self, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+        return tuple(f(self.theta).to(dtype=dtype).contiguous() for f in (torch.cos, torch.sin))
+
+    def _append(self, x, at: tuple, k_past: torch.Tensor, v_past: torch.Tensor):
+        """Heads (B, L, H*Dh) of x's tokens over past and new keys, and the two
+        concatenated; at: addresses of the new tokens' q, k (roped), v and
+        lambda, token-major without gaps, of the RoPE tables and the noise
+        angles' cos and sin."""
+        B, L, D = x.shape
+        H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
+        past, lib, dev = k_past.shape[2], _hip.lib(), x.device
+        w = self.head_norm.weight.detach().to(x.dtype).contiguous() if self.head_norm_mode == "full" else None
+        heads = torch.empty((B, L, D), dtype=x.dtype, device=dev)
+        k, v = (torch.empty((B, Hkv, past + L, Dh), dtype=x.dtype, device=dev) for _ in range(2))
+        q_p, k_p, v_p, l_p, rc_p, rs_p, tc_p, ts_p = at
+        a = _hip.AttnDesc()
+        a.dtype = _hip.dtype_code(x.dtype)
+        a.B, a.H, a.Hkv, a.Lq, a.Dh = B, H, Hkv, L, Dh
         a.q, a.q_sb, a.q_sh, a.q_sl = q_p, L * D, Dh, D
         a.theta_cos, a.theta_sin = tc_p, ts_p
         a.rope_cos, a.rope_sin, a.rope_interleaved = rc_p, rs_p, int(self.rope_interleaved)
@@ -186,5 +217,5 @@ class CoDAGQA(RowsMixin, nn.Module):
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
         a.workspace, a.workspace_bytes = _hip.ptr(ws), need.value
         _hip.check(lib.coda_attn_append(a, k.data_ptr(), v.data_ptr(), Hkv * (past + L) * Dh, (past + L) * Dh, Dh,
-                                        stream))
-        return self._out_rows(heads), (k, v)
+                                        _hip.stream_of(heads)))
+        return heads, (k, v)

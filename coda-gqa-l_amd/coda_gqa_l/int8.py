@@ -8,7 +8,7 @@ the product of two sets of them.
   Int8Rows       - the codes and scales that these hand on
 
 The layers run their projections on them after use_int8_projections()
-(Int8Mixin).  Inference only: no output carries a gradient.  Errors surface
+(Int8Mixin), and take Int8Rows in place of a tensor.  Inference only: no output carries a gradient.  Errors surface
 as RuntimeError, like those of the other operators.
 """
 
@@ -17,8 +17,10 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.nn as nn
 
 from . import _hip
+from .rows import _Made, _capturing
 
 __all__ = ["Int8Rows", "quantize_rows", "rms_norm_int8", "linear_int8"]
 
@@ -222,3 +224,120 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
     _call(_hip.lib().coda_linear_int8, a, _hip.dtype_code(dt), a.data_ptr(), am, sa.data_ptr(), sa.numel(), b.data_ptr(),
           bm, sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
     return out
+
+
+class Int8Mixin:
+    """The projections of a layer in 8 bits: RowsMixin's attributes, and
+    _rope_tables."""
+
+    int8_projections = False
+
+    def use_int8_projections(self, on: bool = True) -> "Int8Mixin":
+        """Run q / k / v / lambda / gate (one product, with the RoPE of k and
+        the sigmoids) and o_proj on 8-bit rows: weights with a scale for each
+        output channel, tokens with a scale each.  Results differ from the
+        float projections' by the roundings to 8 bits.  The float parameters
+        stay; the codes are made of them at the next call and again whenever
+        torch counts a change of one (drop_parameter_copies() after one that
+        it does not count; a captured graph keeps the codes of its capture).
+        The projections have to be plain nn.Linear without hooks."""
+        self.int8_projections = bool(on)
+        self.__dict__.pop("_fast", None)
+        return self
+
+    def _int8_on(self, x) -> bool:
+        """Whether a call on x runs on 8-bit rows."""
+        if isinstance(x, Int8Rows):
+            if not self.int8_projections:
+                raise RuntimeError("the layer takes Int8Rows after use_int8_projections()")
+            return True
+        return self.int8_projections
+
+    def _int8_linears(self) -> list:
+        names = ("q_proj", "k_proj", "v_proj", "lambda_proj") + (("write_proj",) if self._has_gate() else ()) + ("o_proj",)
+        H, Hkv, Dh, D = self.num_heads, self.num_kv_heads, self.head_dim, self.embed_dim
+        shapes = dict(q_proj=(H * Dh, D), k_proj=(Hkv * Dh, D), v_proj=(Hkv * Dh, D), lambda_proj=(H, D), write_proj=(1, D),
+                      o_proj=(D, H * Dh))
+        lins = []
+        for n in names:
+            m = self._modules[n]
+            if type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__ or \
+                    tuple(m.weight.shape) != shapes[n]:
+                raise RuntimeError(f"8-bit projections need {n} to be a plain nn.Linear {shapes[n]} without hooks")
+            lins.append(m)
+        return lins
+
+    def _int8_weights(self) -> Tuple[torch.Tensor, ...]:
+        """(codes, scales, fp32 biases) of q | k | v | lambda | gate in the
+        front end's row order, (codes, scales, bias) of o_proj; kept while the
+        parameters are what they were."""
+        lins = self._int8_linears()
+        ps = [t for m in lins for t in (m.weight, m.bias) if t is not None]
+        tag = tuple((id(t), t._version, t.data_ptr(), t.dtype, t.device) for t in ps) + (self.rope_interleaved,)
+        hit = self.__dict__.get("_int8_made")
+        if hit is not None and hit[0] == tag:
+            hit[2].use()
+            return self._handed(hit[1])
+        Dh, dev = self.head_dim, lins[0].weight.device
+        with torch.no_grad():
+            rows = [quantize_rows(m.weight) for m in lins[:-1]]
+            codes, scales = [r.codes for r in rows], [r.scales for r in rows]
+            bias = [torch.zeros(m.out_features, device=dev) if m.bias is None else m.bias.float() for m in lins[:-1]]
+            if not self.rope_interleaved:
+                # k rows of a head by RoPE pairs (i, i + Dh/2)
+                half = torch.arange(Dh // 2, device=dev)
+                perm = (torch.arange(self.num_kv_heads, device=dev)[:, None] * Dh +
+                        torch.stack([half, half + Dh // 2], 1).reshape(1, -1)).reshape(-1)
+                for part in (codes, scales, bias):
+                    part[1] = part[1][perm]
+            n = sum(m.out_features for m in lins[:-1])
+            out = quantize_rows(lins[-1].weight)
+            val = (torch.cat(codes), torch.cat(scales), torch.cat(bias + [torch.zeros(-n % 4, device=dev)]), out.codes,
+                   out.scales, lins[-1].bias)
+        if not _capturing():
+            self.__dict__["_int8_made"] = (tag, val, _Made(*val[:5]))
+        return val
+
+    def _int8_tokens(self, x) -> Int8Rows:
+        r = x if isinstance(x, Int8Rows) else quantize_rows(x)
+        if r.codes.dim() != 3 or r.cols != self.embed_dim:
+            raise RuntimeError(f"tokens {tuple(r.shape)} are not (B, L, {self.embed_dim})")
+        return r
+
+    def _front_int8(self, x, p0: int):
+        """q (B,H,L,Dh) before RoPE, k (B,Hkv,L,Dh) roped, v, the gate (B,L)
+        float32 (None without one), lambda (B,H,L) and the RoPE tables of
+        positions p0 .., of x (B,L,D), a tensor or Int8Rows."""
+        r = self._int8_tokens(x)
+        B, L, _ = r.shape
+        H, Hkv, Dh, dt, dev = self.num_heads, self.num_kv_heads, self.head_dim, r.dtype, r.device
+        w, sw, bias = self._int8_weights()[:3]
+        if w.device != dev:
+            raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
+        cos, sin = self._rope_tables(p0, L, dev, dt)
+        Fq, Fk = H * Dh, Hkv * Dh
+        q = torch.empty((B, L, H, Dh), dtype=dt, device=dev)
+        k = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
+        v = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
+        lam = torch.empty((B, L, H), dtype=dt, device=dev)
+        g = torch.empty((B, L), dtype=torch.float32, device=dev) if self._has_gate() else None
+        codes, sm, scales = _flat(r)
+        d = self._int8_desc(r, cos, sin, w, bias)
+        d.x, d.x_sm = codes.data_ptr(), sm
+        d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q.data_ptr(), Fq, k.data_ptr(), Fk, v.data_ptr(), Fk
+        d.lam, d.lam_sm, d.g = lam.data_ptr(), H, _hip.ptr(g)
+        _call(_hip.lib().coda_project_int8, codes, d, scales.data_ptr(), sw.data_ptr(), w.stride(0), w.shape[1])
+        return (q.permute(0, 2, 1, 3), k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3), g, lam.permute(0, 2, 1), cos, sin)
+
+    def _int8_desc(self, r: Int8Rows, cos, sin, w: torch.Tensor, bias: torch.Tensor):
+        B, L, _ = r.shape
+        d = self._proj_desc(r, B * L, L, cos, sin)
+        d.w, d.bias = w.data_ptr(), bias.data_ptr()
+        return d
+
+    def _out_proj(self, heads: torch.Tensor) -> torch.Tensor:
+        """o_proj of heads (B, L, H*Dh): the module, or in 8 bits."""
+        if not self.int8_projections:
+            return self.o_proj(heads)
+        w, sw, bias = self._int8_weights()[3:]
+        return linear_int8(quantize_rows(heads), _made(w, sw, heads.shape[-1], heads.dtype), bias)

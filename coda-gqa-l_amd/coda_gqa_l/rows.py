@@ -56,7 +56,7 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
 
 # What a layer keeps between calls: copies derived from parameters; and
 # workspaces, plans and buffers
-_PARAM_COPIES = ("_derived_cache", "_rope_cache", "_rope_made", "_proj_made", "_fast", "_dplan")
+_PARAM_COPIES = ("_derived_cache", "_rope_cache", "_rope_made", "_proj_made", "_fast", "_dplan", "_int8_made")
 _KEPT = _PARAM_COPIES + ("_graph_held", "_step_ws_bytes", "_route_ws", "_route_tag", "_ws_cache", "_block_ws",
                          "_block_checked", "_status_pending", "_snap_cache", "_last_chunk_group")
 
@@ -78,8 +78,9 @@ class RowsMixin:
         Counted changes need no such call.  Prompts, unbounded layers, o_proj,
         fp32 steps and steps of more than 64 rows read the projections' own
         values in any case; kept are the packed q / k / v / lambda / gate
-        weights and RoPE rows of bf16 steps of up to 64 rows, and a bounded
-        layer's noise angles, head norm weight and summary rates."""
+        weights and RoPE rows of bf16 steps of up to 64 rows, the codes of
+        8-bit projections, and a bounded layer's noise angles, head norm
+        weight and summary rates."""
         for k in _PARAM_COPIES:
             self.__dict__.pop(k, None)
 
