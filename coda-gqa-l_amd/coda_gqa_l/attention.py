@@ -502,7 +502,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
             d.rope_cos = a.rope_cos = cos_t.data_ptr() + row
             d.rope_sin = a.rope_sin = sin_t.data_ptr() + row
             if int8:
-                _hip.check(fp["project"](fp["proj_ref"], scales.data_ptr(), *fp["int8_args"], stream))
+                _hip.check(fp["project"](fp["proj_ref"], scales.data_ptr(), *fp["int8_args"], None, stream))
             else:
                 _hip.check(fp["project"](fp["proj_ref"], stream))
         else:

@@ -153,20 +153,7 @@ class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
         buf = torch.empty(at[-1], dtype=torch.uint8, device=dev)
         q_p, k_p, v_p, l_p, g_p, rc_p, rs_p, tc_p, ts_p = (buf.data_ptr() + o for o in at[:-1])
         p = self._proj_params(rows)
-        angles, th, keep = self._angles_rows(dev, past, L), self.theta, ()
-        if angles is not None:
-            p.inv_freq, p.inv_dtype = angles
-            p.p0, p.rope_cos, p.rope_sin = past, rc_p, rs_p
-        else:
-            keep = self._rope_tables(past, L, dev, x.dtype)
-            rc_p, rs_p = (t.data_ptr() for t in keep)
-        if th.dtype in (torch.float32, torch.bfloat16) and th.device == dev and th.shape == (H, half) and \
-                th.is_contiguous():
-            p.theta, p.theta_dtype, p.theta_cos, p.theta_sin = th.data_ptr(), _hip.dtype_code(th.dtype), tc_p, ts_p
-        else:
-            tt = self._theta_pair(x.dtype)
-            tc_p, ts_p = (t.data_ptr() for t in tt)
-            keep += tt
+        (rc_p, rs_p, tc_p, ts_p), keep = self._launch_tables(p, x, past, (rc_p, rs_p, tc_p, ts_p))
         d = self._proj_desc(x, M, L)
         d.rope_cos, d.rope_sin = rc_p, rs_p
         d.x, d.x_sm = xs.data_ptr(), D
@@ -178,10 +165,42 @@ class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
 
     def _decode_int8(self, x, k_past: torch.Tensor, v_past: torch.Tensor):
         """_decode with 8-bit projections."""
-        q, k, v, _, lam, cos, sin = self._front_int8(x, k_past.shape[2])
-        keep = (q, k, v, lam, cos, sin, *self._theta_pair(x.dtype))
-        heads, kv = self._append(x, tuple(t.data_ptr() for t in keep), k_past, v_past)
+        B, L, _ = x.shape
+        past, half, p = k_past.shape[2], self.head_dim // 2, None
+        tables = tuple(torch.empty((n, half), dtype=x.dtype, device=x.device)
+                       for n in (L, L, self.num_heads, self.num_heads))
+        if B * L <= 128:  # (as many rows as a launch makes tables for)
+            p = _hip.ProjParams()
+            at, keep = self._launch_tables(p, x, past, tuple(t.data_ptr() for t in tables))
+        else:
+            tables = (*self._rope_tables(past, L, x.device, x.dtype), *self._theta_pair(x.dtype))
+            at = tuple(t.data_ptr() for t in tables)
+        q, k, v, _, lam, _, _ = self._front_int8(x, past, (p, *at[:2]))
+        heads, kv = self._append(x, (*(t.data_ptr() for t in (q, k, v, lam)), *at), k_past, v_past)
         return self._out_proj(heads), kv
+
+    def _launch_tables(self, p, x, p0: int, at: tuple):
+        """Has the projection's launch make, at these addresses, the RoPE
+        tables of x's tokens from position p0 and the noise angles' cos and sin
+        (p's part of it); where it cannot, makes them here.  Their addresses,
+        and the tensors that hold the latter."""
+        L, dev, dtype, th, keep = x.shape[1], x.device, x.dtype, self.theta, ()
+        rc_p, rs_p, tc_p, ts_p = at
+        angles = self._angles_rows(dev, p0, L)
+        if angles is not None:
+            p.inv_freq, p.inv_dtype = angles
+            p.p0, p.rope_cos, p.rope_sin = p0, rc_p, rs_p
+        else:
+            keep = self._rope_tables(p0, L, dev, dtype)
+            rc_p, rs_p = (t.data_ptr() for t in keep)
+        if th.dtype in (torch.float32, torch.bfloat16) and th.device == dev and \
+                th.shape == (self.num_heads, self.head_dim // 2) and th.is_contiguous():
+            p.theta, p.theta_dtype, p.theta_cos, p.theta_sin = th.data_ptr(), _hip.dtype_code(th.dtype), tc_p, ts_p
+        else:
+            tt = self._theta_pair(dtype)
+            tc_p, ts_p = (t.data_ptr() for t in tt)
+            keep += tt
+        return (rc_p, rs_p, tc_p, ts_p), keep
 
     def _theta_pair(self, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         return tuple(f(self.theta).to(dtype=dtype).contiguous() for f in (torch.cos, torch.sin))

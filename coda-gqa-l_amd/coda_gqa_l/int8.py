@@ -304,17 +304,19 @@ class Int8Mixin:
             raise RuntimeError(f"tokens {tuple(r.shape)} are not (B, L, {self.embed_dim})")
         return r
 
-    def _front_int8(self, x, p0: int):
+    def _front_int8(self, x, p0: int, tables: Optional[tuple] = None):
         """q (B,H,L,Dh) before RoPE, k (B,Hkv,L,Dh) roped, v, the gate (B,L)
         float32 (None without one), lambda (B,H,L) and the RoPE tables of
-        positions p0 .., of x (B,L,D), a tensor or Int8Rows."""
+        positions p0 .., of x (B,L,D), a tensor or Int8Rows.  tables: made by
+        the launch or given, as (coda_proj_params or None, address of cos, of
+        sin)."""
         r = self._int8_tokens(x)
         B, L, _ = r.shape
         H, Hkv, Dh, dt, dev = self.num_heads, self.num_kv_heads, self.head_dim, r.dtype, r.device
         w, sw, bias = self._int8_weights()[:3]
         if w.device != dev:
             raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
-        cos, sin = self._rope_tables(p0, L, dev, dt)
+        cos, sin = self._rope_tables(p0, L, dev, dt) if tables is None else (None, None)
         Fq, Fk = H * Dh, Hkv * Dh
         q = torch.empty((B, L, H, Dh), dtype=dt, device=dev)
         k = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
@@ -322,18 +324,17 @@ class Int8Mixin:
         lam = torch.empty((B, L, H), dtype=dt, device=dev)
         g = torch.empty((B, L), dtype=torch.float32, device=dev) if self._has_gate() else None
         codes, sm, scales = _flat(r)
-        d = self._int8_desc(r, cos, sin, w, bias)
+        d = self._proj_desc(r, B * L, L, cos, sin)
+        params = None
+        if tables is not None:
+            params, d.rope_cos, d.rope_sin = tables
+        d.w, d.bias = w.data_ptr(), bias.data_ptr()
         d.x, d.x_sm = codes.data_ptr(), sm
         d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q.data_ptr(), Fq, k.data_ptr(), Fk, v.data_ptr(), Fk
         d.lam, d.lam_sm, d.g = lam.data_ptr(), H, _hip.ptr(g)
-        _call(_hip.lib().coda_project_int8, codes, d, scales.data_ptr(), sw.data_ptr(), w.stride(0), w.shape[1])
+        _call(_hip.lib().coda_project_int8, codes, d, scales.data_ptr(), sw.data_ptr(), w.stride(0), w.shape[1],
+              params)
         return (q.permute(0, 2, 1, 3), k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3), g, lam.permute(0, 2, 1), cos, sin)
-
-    def _int8_desc(self, r: Int8Rows, cos, sin, w: torch.Tensor, bias: torch.Tensor):
-        B, L, _ = r.shape
-        d = self._proj_desc(r, B * L, L, cos, sin)
-        d.w, d.bias = w.data_ptr(), bias.data_ptr()
-        return d
 
     def _out_proj(self, heads: torch.Tensor) -> torch.Tensor:
         """o_proj of heads (B, L, H*Dh): the module, or in 8 bits."""

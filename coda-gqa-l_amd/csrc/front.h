@@ -39,6 +39,23 @@ struct FrontTables {
   void* theta_sin;
 };
 
+// What a launch leaves of its own tables, by 512 threads
+template <typename T>
+__device__ __forceinline__ void leave_tables(const FrontTables& tab, int L, int half, int t) {
+  if (tab.inv_freq)
+    for (int i = t; i < L * half; i += 512) {
+      const float2 a = rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + i / half, i % half);
+      ((T*)tab.rope_cos)[i] = Elt<T>::st(a.x);
+      ((T*)tab.rope_sin)[i] = Elt<T>::st(a.y);
+    }
+  if (tab.theta)
+    for (int i = t; i < tab.n_theta; i += 512) {
+      const float2 a = cos_sin_of<T>(angle_ld(tab.theta, tab.theta_dtype, i), tab.theta_dtype);
+      ((T*)tab.theta_cos)[i] = Elt<T>::st(a.x);
+      ((T*)tab.theta_sin)[i] = Elt<T>::st(a.y);
+    }
+}
+
 // Epilogue of features f .. f + 3 (f a multiple of 4) of token row m:
 // the fp32 accumulators plus bias, rounded and routed to q / k (RoPE) / v /
 // lambda / gate
@@ -118,21 +135,7 @@ struct FrontEpilogue {
   // no gate column: the gate is 1; the tables that the launch leaves
   __device__ __forceinline__ void once(int t) const {
     if (!d.gate && t < d.M) d.g[t] = 1.f;
-    if constexpr (PARAMS) {
-      const int half = d.Dh / 2;
-      if (tab.inv_freq)
-        for (int i = t; i < d.L * half; i += 512) {
-          const float2 a = rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + i / half, i % half);
-          ((T*)tab.rope_cos)[i] = Elt<T>::st(a.x);
-          ((T*)tab.rope_sin)[i] = Elt<T>::st(a.y);
-        }
-      if (tab.theta)
-        for (int i = t; i < tab.n_theta; i += 512) {
-          const float2 a = cos_sin_of<T>(angle_ld(tab.theta, tab.theta_dtype, i), tab.theta_dtype);
-          ((T*)tab.theta_cos)[i] = Elt<T>::st(a.x);
-          ((T*)tab.theta_sin)[i] = Elt<T>::st(a.y);
-        }
-    }
+    if constexpr (PARAMS) leave_tables<T>(tab, d.L, d.Dh / 2, t);
   }
 };
 

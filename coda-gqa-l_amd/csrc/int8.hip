@@ -288,6 +288,7 @@ struct LinearSink {
     T* p;
     int n;
   };
+  __device__ __forceinline__ void once(int) const {}
   __device__ __forceinline__ float bias1(int f) const { return bias ? Elt<T>::ld(bias[f]) : 0.f; }
   __device__ __forceinline__ Lane lane(int f) const { return Lane{out + f, n_feat - f}; }
   template <int N>
@@ -306,24 +307,103 @@ struct LinearSink {
   }
 };
 
-// The projection front end (FrontEpilogue, its bias added already)
-struct NoBias {
-  __device__ __forceinline__ pf32x4 bias4(int, int) const { return pf32x4{0.f, 0.f, 0.f, 0.f}; }
+// n / d for n below 2^31 without a division (d's reciprocal of 33 bits, from
+// the host)
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(int div) : d((uint32_t)div) {
+    shift = 0;
+    while ((1u << shift) < d) ++shift;
+    mul = (uint32_t)(((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t mod(uint32_t n) const {
+    const uint32_t h = __umulhi(mul, n), q = shift ? (h + ((n - h) >> 1)) >> (shift - 1) : n;
+    return n - q * d;
+  }
 };
-template <typename T>
+
+// The projection front end: the sections and roundings of FrontEpilogue (a
+// value is rounded to T before the RoPE or the sigmoid), with all that does
+// not change from token to token found once.  TABLES: angles that the launch
+// makes itself where tab says so.
+template <typename T, bool TABLES>
 struct FrontSink {
   typedef T Out;
+  typedef Elt<T> E;
   static constexpr int kRun = 4;
-  FrontEpilogue<T, true> epi;
+  coda_proj_desc d;
+  FrontTables tab;
+  FastDiv len;  // of a sequence: table row = token % L
   int n_feat;
+  // Where four features go: q or v (kind 0), k (1), single lambdas / gates
+  // (2); at: of a token 0's first channel (kind 1: of its head), c: that
+  // channel (kind 2: the feature)
   struct Lane {
-    int f;
+    int kind, c;
+    T* at;
+    int64_t sm;
   };
-  __device__ __forceinline__ float bias1(int f) const { return epi.d.bias[f]; }
-  __device__ __forceinline__ Lane lane(int f) const { return Lane{f}; }
+  __device__ __forceinline__ float bias1(int f) const { return d.bias[f]; }
+  __device__ __forceinline__ Lane lane(int f) const {
+    const int Fq = d.H * d.Dh, Fk = d.Hkv * d.Dh;
+    if (f < Fq) return Lane{0, 0, (T*)d.q + f, d.q_sm};
+    if (f < Fq + Fk) {
+      const int c = (f - Fq) % d.Dh;
+      return Lane{1, c, (T*)d.k + (f - Fq - c), d.k_sm};
+    }
+    if (f < Fq + 2 * Fk) return Lane{0, 0, (T*)d.v + (f - Fq - Fk), d.v_sm};
+    return Lane{2, f, nullptr, 0};
+  }
   __device__ __forceinline__ void put(const Lane& l, int m, const Feats<T, 4>& v) const {
-    using E = Elt<T>;
-    epi(NoBias{}, l.f, m, pf32x4{E::ld(v.v[0]), E::ld(v.v[1]), E::ld(v.v[2]), E::ld(v.v[3])});
+    // (8-byte rows: see the entry's checks)
+    typedef uint32_t V __attribute__((ext_vector_type(sizeof(T)), aligned(8)));  // four T
+    struct alignas(2 * sizeof(T)) Two {
+      T v[2];
+    };
+    if (l.kind == 0) {
+      *reinterpret_cast<V*>(l.at + (int64_t)m * l.sm) = __builtin_bit_cast(V, v);
+    } else if (l.kind == 1) {
+      const int half = d.Dh / 2, p = l.c / 2;
+      const int prow = (int)len.mod((uint32_t)m);
+      const bool inter = d.rope_interleaved != 0;
+      const T* cs = (const T*)d.rope_cos + (int64_t)prow * half + p;
+      const T* sn = (const T*)d.rope_sin + (int64_t)prow * half + p;
+      float r[4];
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp) {
+        float cc, ss;
+        if (TABLES && tab.inv_freq) {
+          const float2 a = rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + prow, p + pp);
+          cc = a.x;
+          ss = a.y;
+        } else {
+          cc = E::ld(cs[pp]);
+          ss = E::ld(sn[pp]);
+        }
+        rope_pair_t<T>(E::ld(v.v[2 * pp]), E::ld(v.v[2 * pp + 1]), cc, ss, inter, r[2 * pp], r[2 * pp + 1]);
+      }
+      T* row = l.at + (int64_t)m * l.sm;
+      if (inter) {
+        const Feats<T, 4> o{{E::st(r[0]), E::st(r[1]), E::st(r[2]), E::st(r[3])}};
+        *reinterpret_cast<V*>(row + l.c) = __builtin_bit_cast(V, o);
+      } else {  // pairs (p, p + half): channels p, p + 1 and the same + half
+        *reinterpret_cast<Two*>(row + p) = Two{{E::st(r[0]), E::st(r[2])}};
+        *reinterpret_cast<Two*>(row + p + half) = Two{{E::st(r[1]), E::st(r[3])}};
+      }
+    } else {
+      const int o_l = d.H * d.Dh + 2 * d.Hkv * d.Dh, o_g = o_l + d.H;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int f = l.c + e;
+        if (f >= n_feat) continue;
+        const float sg = E::rnd(proj_sigmoid(E::ld(v.v[e])));
+        if (f < o_g) ((T*)d.lam)[(int64_t)m * d.lam_sm + (f - o_l)] = E::st(sg);
+        else d.g[m] = sg;
+      }
+    }
+  }
+  __device__ __forceinline__ void once(int t) const {
+    if constexpr (TABLES) leave_tables<T>(tab, d.L, d.Dh / 2, t);
   }
 };
 
@@ -626,14 +706,17 @@ struct RowsSink {
     }
     sink.put(sink.lane(f), m, int8_value<typename Sink::Out>(a, sx[m], s, b));
   }
-  __device__ __forceinline__ void once(int) const {}
+  __device__ __forceinline__ void once(int t) const { sink.once(t); }
 };
 
+static constexpr int kFewRows = 128;
 template <typename Sink>
-static int launch_int8(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  if (X.rows <= 128)
-    return launch_rows<int8_t>(MatRows<int8_t>{W.p, W.sm}, W.rows, K, X.p, X.sm, X.rows,
-                               RowsSink<Sink>{sink, X.scales, W.scales, W.rows}, st, who);
+static int launch_few(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
+  return launch_rows<int8_t>(MatRows<int8_t>{W.p, W.sm}, W.rows, K, X.p, X.sm, X.rows,
+                             RowsSink<Sink>{sink, X.scales, W.scales, W.rows}, st, who);
+}
+template <typename Sink>
+static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
   // the largest tile that gives every CU one
   const int cus = device_cus();
   auto tiles = [&](int b) { return ((int64_t)W.rows + b - 1) / b * (((int64_t)X.rows + b - 1) / b); };
@@ -724,13 +807,15 @@ extern "C" int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const 
   if (rc || M == 0) return rc;
   CODA_REQUIRE(out && o_sm >= n_feat, "%s: no output, or its rows shorter than %d features", who, n_feat);
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T) launch_int8(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who)
+#define RUN(T)                                                              \
+  (M <= kFewRows ? launch_few(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who) \
+                 : launch_many(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who))
   return dtype == CODA_F32 ? RUN(float) : dtype == CODA_BF16 ? RUN(bf16_t) : RUN(f16_t);
 #undef RUN
 }
 
 extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales, const float* w_scales, int64_t w_sm,
-                                 int K, void* stream) {
+                                 int K, const coda_proj_params* p, void* stream) {
   const char* who = "coda_project_int8";
   CODA_REQUIRE(d != nullptr, "%s: null descriptor", who);
   CODA_REQUIRE(d->dtype == CODA_BF16 || d->dtype == CODA_F32, "%s: dtype must be CODA_F32 or CODA_BF16", who);
@@ -740,14 +825,29 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
   const Int8Mat X{(const int8_t*)d->x, d->x_sm, x_scales, d->M}, W{(const int8_t*)d->w, w_sm, w_scales, n_feat};
   const int rc = check_mats(X, W, K, who);
   if (rc || d->M == 0) return rc;
-  CODA_REQUIRE(d->bias && d->rope_cos && d->rope_sin && d->q && d->k && d->v && d->lam && (d->g || !d->gate),
+  const bool own = p && p->inv_freq;
+  CODA_REQUIRE(d->bias && (own || (d->rope_cos && d->rope_sin)) && d->q && d->k && d->v && d->lam && (d->g || !d->gate),
                "%s: pointer missing", who);
   CODA_REQUIRE(((uintptr_t)d->bias % 16) == 0, "%s: bias must be 16-byte aligned", who);
   CODA_REQUIRE(d->q_sm % 4 == 0 && d->k_sm % 4 == 0 && d->v_sm % 4 == 0 && ((uintptr_t)d->q % 8) == 0 &&
                    ((uintptr_t)d->k % 8) == 0 && ((uintptr_t)d->v % 8) == 0,
                "%s: q / k / v rows must be 8-byte aligned", who);
+  FrontTables tab{};
+  if (p) {
+    const auto angle = [](int t) { return t == CODA_F32 || t == CODA_BF16; };
+    CODA_REQUIRE(!own || (p->rope_cos && p->rope_sin && angle(p->inv_dtype) && p->p0 >= 0 && p->p0 + d->L <= 1 << 24),
+                 "%s: RoPE tables missing, or positions past 2^24", who);
+    CODA_REQUIRE(!p->theta || (p->theta_cos && p->theta_sin && angle(p->theta_dtype)), "%s: theta tables missing", who);
+    CODA_REQUIRE(d->M <= kFewRows, "%s: a launch makes the tables of at most %d token rows, not of %d", who, kFewRows,
+                 d->M);
+    tab = FrontTables{p->inv_freq,   p->inv_dtype, p->p0,        p->rope_cos, p->rope_sin, p->theta,
+                      p->theta_dtype, d->H * (d->Dh / 2), p->theta_cos, p->theta_sin};
+  }
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T) launch_int8(X, W, K, FrontSink<T>{{*d, FrontTables{}}, n_feat}, st, who)
+  const FastDiv len(d->L);
+#define RUN(T)                                                                        \
+  (d->M <= kFewRows ? launch_few(X, W, K, FrontSink<T, true>{*d, tab, len, n_feat}, st, who) \
+                    : launch_many(X, W, K, FrontSink<T, false>{*d, tab, len, n_feat}, st, who))
   return d->dtype == CODA_BF16 ? RUN(bf16_t) : RUN(float);
 #undef RUN
 }

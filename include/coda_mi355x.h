@@ -224,9 +224,10 @@ int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const float* x_sc
  * of token rows: d->x (M, K) and d->w (n_feat, K) are codes (d->x_sm and w_sm
  * in bytes, w row-major in coda_project's row order; D and w_layout unused),
  * dtype CODA_BF16 or CODA_F32 the type of q, k, v, lam and the tables.
- * gate == 0 leaves g alone (it may be NULL). */
+ * gate == 0 leaves g alone (it may be NULL).  p may be NULL; of it only the
+ * tables are read, as in coda_project_params (at most 128 token rows then). */
 int coda_project_int8(const coda_proj_desc* d, const float* x_scales, const float* w_scales, int64_t w_sm, int K,
-                      void* stream);
+                      const coda_proj_params* p, void* stream);
 
 
 

@@ -105,6 +105,25 @@ def test_project_entry(change, error):
                           q=P, q_sm=128, k=P, k_sm=64, v=P, v_sm=64, lam=P, lam_sm=2, g=P), **change).items():
         setattr(d, n, v)
     L = _hip.lib()
-    assert L.coda_project_int8(d, P, P, 128, 128, None) == 1
+    assert L.coda_project_int8(d, P, P, 128, 128, None, None) == 1
     assert error in L.coda_last_error().decode()
-    assert L.coda_project_int8(None, P, P, 128, 128, None) == 1
+    assert L.coda_project_int8(None, P, P, 128, 128, None, None) == 1
+
+
+@pytest.mark.parametrize("dim,params,error", [
+    (dict(M=129), dict(inv_freq=P, rope_cos=P, rope_sin=P), "at most 128"),
+    (dict(), dict(inv_freq=P, rope_cos=P), "RoPE tables"),
+    (dict(), dict(inv_freq=P, rope_cos=P, rope_sin=P, inv_dtype=2), "RoPE tables"),
+    (dict(), dict(inv_freq=P, rope_cos=P, rope_sin=P, p0=1 << 24), "2^24"),
+    (dict(), dict(theta=P, theta_cos=P), "theta tables"),
+])
+def test_project_entry_tables(dim, params, error):
+    d, p = _hip.ProjDesc(), _hip.ProjParams()
+    for n, v in dict(dict(dtype=1, M=2, L=1, H=2, Hkv=1, Dh=64, gate=1, x=P, x_sm=128, w=P, bias=P, rope_cos=P, rope_sin=P,
+                          q=P, q_sm=128, k=P, k_sm=64, v=P, v_sm=64, lam=P, lam_sm=2, g=P), **dim).items():
+        setattr(d, n, v)
+    for n, v in params.items():
+        setattr(p, n, v)
+    L = _hip.lib()
+    assert L.coda_project_int8(d, P, P, 128, 128, p, None) == 1
+    assert error in L.coda_last_error().decode()
