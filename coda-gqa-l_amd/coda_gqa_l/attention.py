@@ -526,7 +526,18 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
         fp["record_pos"] = pos + 1 if routed.value else -1
         # the general path's carried-record tag no longer matches this state
         self.__dict__["_route_tag"] = None
-        return self._out_proj(fp["heads_flat"]) if int8 else self._out_rows(fp["heads_flat"], kept=True)
+        return self._step_int8_out(fp, stream) if int8 else self._out_rows(fp["heads_flat"], kept=True)
+
+    def _step_int8_out(self, fp: dict, stream: int) -> torch.Tensor:
+        """_out_proj of a cached step's heads."""
+        heads, (codes, scales, w, sw, bias) = fp["heads_flat"], fp["int8_out"]
+        B, _, F = heads.shape
+        y = torch.empty((B, 1, w.shape[0]), dtype=heads.dtype, device=heads.device)
+        lib, dt, P = _hip.lib(), fp["proj"].dtype, codes.shape[1]
+        _hip.check(lib.coda_quantize_rows(dt, heads.data_ptr(), F, B, F, codes.data_ptr(), P, scales.data_ptr(), stream))
+        _hip.check(lib.coda_linear_int8(dt, codes.data_ptr(), P, scales.data_ptr(), B, w.data_ptr(), P, sw.data_ptr(),
+                                        w.shape[0], P, _hip.ptr(bias), y.data_ptr(), w.shape[0], stream))
+        return y
 
     def _step_int8_tokens(self, fp: dict, d, x, stream: int) -> torch.Tensor:
         """The tokens of a cached step in 8 bits: their codes in d, their scales."""
@@ -585,16 +596,18 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
             cos_t, sin_t = torch.empty((2, 1, Dh // 2), dtype=dt, device=dev)
             row = slice(0, 1)
         d = self._proj_desc(x, B, 1, cos_t, sin_t)
-        int8_args = int8_tokens = None
+        int8_args = int8_tokens = int8_out = None
         if int8:
             if D != self.embed_dim:
                 return None
-            w, sw, b = self._int8_weights()[:3]
+            w, sw, b, ow, osw, ob = self._int8_weights()
             if w.device != dev:
                 raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
             d.w, d.bias, int8_args = w.data_ptr(), b.data_ptr(), (sw.data_ptr(), w.stride(0), w.shape[1])
             int8_tokens = (torch.empty((B, w.shape[1]), dtype=torch.int8, device=dev),
                            torch.empty(B, dtype=torch.float32, device=dev))
+            int8_out = (torch.empty((B, ow.shape[1]), dtype=torch.int8, device=dev),
+                        torch.empty(B, dtype=torch.float32, device=dev), ow, osw, ob)
             w = (w, sw)
             if not self._has_gate():
                 g.fill_(1.0)  # the launch leaves it alone
@@ -623,7 +636,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
         routed = ctypes.c_int(0)
 
         fp = {"st": st, "vers": vers, "pvers": pvers, "B": B, "dev": dev, "dtype": dt, "stream": _hip.stream_of(x),
-              "packed": packed, "int8": int8, "int8_args": int8_args, "int8_tokens": int8_tokens, "rows": None,
+              "packed": packed, "int8": int8, "int8_args": int8_args, "int8_tokens": int8_tokens, "int8_out": int8_out,
+              "rows": None,
               "step": L_.coda_decode_step,
               "ptrs": tuple(-1 if t is None else t.data_ptr() for t in ts),
               "tab": (cos_t, sin_t), "row_bytes": (Dh // 2) * cos_t.element_size(),
