@@ -275,7 +275,8 @@ struct alignas(N * sizeof(T)) Feats {
 
 // Where the values of a product go: bias1(f) is added to feature f; lane(f) is
 // what a lane that writes features f .. f + N - 1 of several tokens needs to
-// know once, put() writes them for token m (N = 4, or kRun; f a multiple).
+// know once, put() writes them for tokens m, m + step, .. below rows (N = 4,
+// or kRun; f a multiple).
 template <typename T>
 struct LinearSink {
   typedef T Out;
@@ -291,18 +292,23 @@ struct LinearSink {
   __device__ __forceinline__ void once(int) const {}
   __device__ __forceinline__ float bias1(int f) const { return bias ? Elt<T>::ld(bias[f]) : 0.f; }
   __device__ __forceinline__ Lane lane(int f) const { return Lane{out + f, n_feat - f}; }
-  template <int N>
-  __device__ __forceinline__ void put(const Lane& l, int m, const Feats<T, N>& v) const {
+  template <int N, int R>
+  __device__ __forceinline__ void put(const Lane& l, int m, int step, int rows, const Feats<T, N> (&v)[R]) const {
     // (rows of any element address)
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(2)));
-    typedef typename std::conditional<sizeof(v) == 8, u32x2, pu32x4u>::type V;
+    typedef typename std::conditional<sizeof(v[0]) == 8, u32x2, pu32x4u>::type V;
     T* row = l.p + (int64_t)m * o_sm;
+    const int64_t next = step * o_sm;
     if (l.n >= N) {
-      *reinterpret_cast<V*>(row) = __builtin_bit_cast(V, v);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (m + r * step < rows) *reinterpret_cast<V*>(row + r * next) = __builtin_bit_cast(V, v[r]);
     } else {
 #pragma unroll
-      for (int e = 0; e < N - 1; ++e)
-        if (e < l.n) row[e] = v.v[e];
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e)
+          if (e < l.n && m + r * step < rows) row[r * next + e] = v[r].v[e];
     }
   }
 };
@@ -354,52 +360,63 @@ struct FrontSink {
     if (f < Fq + 2 * Fk) return Lane{0, 0, (T*)d.v + (f - Fq - Fk), d.v_sm};
     return Lane{2, f, nullptr, 0};
   }
-  __device__ __forceinline__ void put(const Lane& l, int m, const Feats<T, 4>& v) const {
+  template <int R>
+  __device__ __forceinline__ void put(const Lane& l, int m, int step, int rows, const Feats<T, 4> (&v)[R]) const {
     // (8-byte rows: see the entry's checks)
     typedef uint32_t V __attribute__((ext_vector_type(sizeof(T)), aligned(8)));  // four T
     struct alignas(2 * sizeof(T)) Two {
       T v[2];
     };
+    T* row = l.at + (int64_t)m * l.sm;
+    const int64_t next = step * l.sm;
     if (l.kind == 0) {
-      *reinterpret_cast<V*>(l.at + (int64_t)m * l.sm) = __builtin_bit_cast(V, v);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (m + r * step < rows) *reinterpret_cast<V*>(row + r * next) = __builtin_bit_cast(V, v[r]);
     } else if (l.kind == 1) {
       const int half = d.Dh / 2, p = l.c / 2;
-      const int prow = (int)len.mod((uint32_t)m);
       const bool inter = d.rope_interleaved != 0;
-      const T* cs = (const T*)d.rope_cos + (int64_t)prow * half + p;
-      const T* sn = (const T*)d.rope_sin + (int64_t)prow * half + p;
-      float r[4];
+      float2 a[R][2];
 #pragma unroll
-      for (int pp = 0; pp < 2; ++pp) {
-        float cc, ss;
-        if (TABLES && tab.inv_freq) {
-          const float2 a = rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + prow, p + pp);
-          cc = a.x;
-          ss = a.y;
-        } else {
-          cc = E::ld(cs[pp]);
-          ss = E::ld(sn[pp]);
-        }
-        rope_pair_t<T>(E::ld(v.v[2 * pp]), E::ld(v.v[2 * pp + 1]), cc, ss, inter, r[2 * pp], r[2 * pp + 1]);
+      for (int r = 0; r < R; ++r) {
+        const int prow = (int)len.mod((uint32_t)min(m + r * step, rows - 1));
+        const T* cs = (const T*)d.rope_cos + (int64_t)prow * half + p;
+        const T* sn = (const T*)d.rope_sin + (int64_t)prow * half + p;
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp)
+          a[r][pp] = TABLES && tab.inv_freq ? rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + prow, p + pp)
+                                            : float2{E::ld(cs[pp]), E::ld(sn[pp])};
       }
-      T* row = l.at + (int64_t)m * l.sm;
-      if (inter) {
-        const Feats<T, 4> o{{E::st(r[0]), E::st(r[1]), E::st(r[2]), E::st(r[3])}};
-        *reinterpret_cast<V*>(row + l.c) = __builtin_bit_cast(V, o);
-      } else {  // pairs (p, p + half): channels p, p + 1 and the same + half
-        *reinterpret_cast<Two*>(row + p) = Two{{E::st(r[0]), E::st(r[2])}};
-        *reinterpret_cast<Two*>(row + p + half) = Two{{E::st(r[1]), E::st(r[3])}};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (m + r * step >= rows) continue;
+        float o[4];
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp)
+          rope_pair_t<T>(E::ld(v[r].v[2 * pp]), E::ld(v[r].v[2 * pp + 1]), a[r][pp].x, a[r][pp].y, inter, o[2 * pp],
+                         o[2 * pp + 1]);
+        T* at = row + r * next;
+        if (inter) {
+          const Feats<T, 4> w{{E::st(o[0]), E::st(o[1]), E::st(o[2]), E::st(o[3])}};
+          *reinterpret_cast<V*>(at + l.c) = __builtin_bit_cast(V, w);
+        } else {  // pairs (p, p + half): channels p, p + 1 and the same + half
+          *reinterpret_cast<Two*>(at + p) = Two{{E::st(o[0]), E::st(o[2])}};
+          *reinterpret_cast<Two*>(at + p + half) = Two{{E::st(o[1]), E::st(o[3])}};
+        }
       }
     } else {
       const int o_l = d.H * d.Dh + 2 * d.Hkv * d.Dh, o_g = o_l + d.H;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = l.c + e;
-        if (f >= n_feat) continue;
-        const float sg = E::rnd(proj_sigmoid(E::ld(v.v[e])));
-        if (f < o_g) ((T*)d.lam)[(int64_t)m * d.lam_sm + (f - o_l)] = E::st(sg);
-        else d.g[m] = sg;
-      }
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int f = l.c + e;
+          const int64_t mr = m + r * step;
+          if (f >= n_feat || mr >= rows) continue;
+          const float sg = E::rnd(proj_sigmoid(E::ld(v[r].v[e])));
+          if (f < o_g) ((T*)d.lam)[mr * d.lam_sm + (f - o_l)] = E::st(sg);
+          else d.g[mr] = sg;
+        }
     }
   }
   __device__ __forceinline__ void once(int t) const {
@@ -659,12 +676,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
         __builtin_amdgcn_wave_barrier();
         const int f = a.f + fw + part * L::kFeats + fq;
         const typename Sink::Lane to = sink.lane(min(f, W.rows - 1));
+        constexpr int R = PR / 2;  // of 32 tokens: 64 / PR a turn
+        Feats<T, N> v[R];
 #pragma unroll
-        for (int r = 0; r < 32; r += 64 / PR) {
-          const int row = r + le / PR, m = a.m + mw + 32 * j + row;
-          const Feats<T, N> v = *reinterpret_cast<const Feats<T, N>*>(mine + row * L::kRow + fq * sizeof(T));
-          if (m < X.rows && f < W.rows) sink.put(to, m, v);
-        }
+        for (int r = 0; r < R; ++r)
+          v[r] = *reinterpret_cast<const Feats<T, N>*>(mine + (r * (64 / PR) + le / PR) * L::kRow + fq * sizeof(T));
+        if (f < W.rows) sink.put(to, a.m + mw + 32 * j + le / PR, 64 / PR, X.rows, v);
         __builtin_amdgcn_wave_barrier();
       });
     });
@@ -704,7 +721,8 @@ struct RowsSink {
       s[e] = sw[g];
       b[e] = sink.bias1(g);
     }
-    sink.put(sink.lane(f), m, int8_value<typename Sink::Out>(a, sx[m], s, b));
+    const Feats<typename Sink::Out, 4> v[1] = {int8_value<typename Sink::Out>(a, sx[m], s, b)};
+    sink.put(sink.lane(f), m, 1, m + 1, v);
   }
   __device__ __forceinline__ void once(int t) const { sink.once(t); }
 };
