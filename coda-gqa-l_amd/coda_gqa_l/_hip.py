@@ -147,7 +147,7 @@ _SIGS = {
     "coda_quantize_rows": (_i32, [_i32, _vp, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
     "coda_rms_norm_int8": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _vp, _vp]),
     "coda_dequantize_rows": (_i32, [_i32, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _vp]),
-    "coda_linear_int8": (_i32, [_i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _vp]),
+    "coda_linear_int8": (_i32, [_i32, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _vp]),
     "coda_project_int8": (_i32, [ctypes.POINTER(ProjDesc), _vp, _vp, _i64, _i32, ctypes.POINTER(ProjParams), _vp]),
     "coda_topk_order_host": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
     # the reference's typed epilogue symbols (void, errors in coda_last_error)

@@ -29,7 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import _hip, ops
-from .int8 import Int8Mixin, Int8Rows, _flat
+from .int8 import FLOAT_ROWS, Int8Mixin, Int8Rows, _flat
 from .memory_banks import METRIC_KEYS, DeviceMetrics, MemoryBankMixin
 from .primitives import HeadwiseRMSNorm, RotaryEmbedding, apply_rope
 from .rows import RowsMixin, _aligned, _capturing, _version
@@ -502,7 +502,7 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
             d.rope_cos = a.rope_cos = cos_t.data_ptr() + row
             d.rope_sin = a.rope_sin = sin_t.data_ptr() + row
             if int8:
-                _hip.check(fp["project"](fp["proj_ref"], scales.data_ptr(), *fp["int8_args"], None, stream))
+                _hip.check(fp["project"](fp["proj_ref"], _hip.ptr(scales), *fp["int8_args"], None, stream))
             else:
                 _hip.check(fp["project"](fp["proj_ref"], stream))
         else:
@@ -533,24 +533,31 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
         heads, (codes, scales, w, sw, bias) = fp["heads_flat"], fp["int8_out"]
         B, _, F = heads.shape
         y = torch.empty((B, 1, w.shape[0]), dtype=heads.dtype, device=heads.device)
-        lib, dt, P = _hip.lib(), fp["proj"].dtype, codes.shape[1]
-        _hip.check(lib.coda_quantize_rows(dt, heads.data_ptr(), F, B, F, codes.data_ptr(), P, scales.data_ptr(), stream))
-        _hip.check(lib.coda_linear_int8(dt, codes.data_ptr(), P, scales.data_ptr(), B, w.data_ptr(), P, sw.data_ptr(),
-                                        w.shape[0], P, _hip.ptr(bias), y.data_ptr(), w.shape[0], stream))
+        lib, dt, P, x = _hip.lib(), fp["proj"].dtype, w.shape[1], (heads.data_ptr(), F, None)
+        if B > FLOAT_ROWS:
+            _hip.check(lib.coda_quantize_rows(dt, heads.data_ptr(), F, B, F, codes.data_ptr(), P, scales.data_ptr(),
+                                              stream))
+            x = codes.data_ptr(), P, scales.data_ptr()
+        _hip.check(lib.coda_linear_int8(dt, *x, B, F, w.data_ptr(), P, sw.data_ptr(), w.shape[0], P, _hip.ptr(bias),
+                                        y.data_ptr(), w.shape[0], stream))
         return y
 
-    def _step_int8_tokens(self, fp: dict, d, x, stream: int) -> torch.Tensor:
-        """The tokens of a cached step in 8 bits: their codes in d, their scales."""
+    def _step_int8_tokens(self, fp: dict, d, x, stream: int) -> Optional[torch.Tensor]:
+        """The tokens of a cached step in d, and the scales where they are in 8
+        bits."""
         if isinstance(x, Int8Rows):
             codes, d.x_sm, scales = _flat(x)
             d.x = codes.data_ptr()
             fp["int8_rows"] = codes
             return scales
+        x = fp["int8_rows"] = _aligned(x)
+        B, _, D = x.shape
+        if B <= FLOAT_ROWS:
+            d.x, d.x_sm = x.data_ptr(), D
+            return None
         codes, scales = fp["int8_tokens"]
-        x = _aligned(x)
         d.x, d.x_sm = codes.data_ptr(), codes.shape[1]
-        _hip.check(_hip.lib().coda_quantize_rows(d.dtype, x.data_ptr(), x.shape[-1], x.shape[0], x.shape[-1], d.x, d.x_sm,
-                                                 scales.data_ptr(), stream))
+        _hip.check(_hip.lib().coda_quantize_rows(d.dtype, x.data_ptr(), D, B, D, d.x, d.x_sm, scales.data_ptr(), stream))
         return scales
 
     def _param_key(self) -> tuple:

@@ -26,6 +26,7 @@ __all__ = ["Int8Rows", "quantize_rows", "rms_norm_int8", "linear_int8"]
 
 PAD = 128        # codes of a row are stored up to a multiple of this
 MAX_ROW = 32768  # longest row that codes are made of
+FLOAT_ROWS = 4  # token rows that a product's launch quantises itself
 
 
 def _padded(cols: int) -> int:
@@ -203,26 +204,38 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     return _made(codes, scales, D, dt), out
 
 
-def linear_int8(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+def linear_int8(x: Union[Int8Rows, torch.Tensor], weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (..., K) times weight (N, K), both in 8 bits: the sum of products is
     exact in int32, then times the token's and the channel's scale, plus bias
-    (N,), rounded once to x's type.  K at most 130944."""
-    if not isinstance(x, Int8Rows) or not isinstance(weight, Int8Rows):
-        raise TypeError("linear_int8 takes Int8Rows (quantize_rows, rms_norm_int8 make them)")
-    wc, dt = weight.codes, x.dtype
-    if wc.dim() != 2 or weight.cols != x.cols or wc.shape[0] == 0:
-        raise RuntimeError(f"linear_int8: weight {tuple(weight.shape)} does not fit x {tuple(x.shape)}")
+    (N,), rounded once to x's type.  K at most 130944.  A tensor x is
+    quantised by rows first (quantize_rows; K at most 32768), up to 4 rows on
+    the product's own way through the weights: the same bits."""
+    if not isinstance(weight, Int8Rows) or not isinstance(x, (Int8Rows, torch.Tensor)):
+        raise TypeError("linear_int8 takes a tensor or Int8Rows, and a weight in Int8Rows (quantize_rows makes them)")
+    wc, dt, shape = weight.codes, x.dtype, x.shape
+    if wc.dim() != 2 or not shape or weight.cols != shape[-1] or wc.shape[0] == 0:
+        raise RuntimeError(f"linear_int8: weight {tuple(weight.shape)} does not fit x {tuple(shape)}")
     N, P = wc.shape
-    a, am, sa = _flat(x)
     b, bm, sb = _flat(weight)
+    sa = None
+    if not isinstance(x, Int8Rows):
+        K = _check_input(x, "linear_int8")
+        M = x.numel() // K
+        if M <= FLOAT_ROWS:
+            a, am = _rows_of(x)
+        else:
+            x = quantize_rows(x)
+    if isinstance(x, Int8Rows):
+        a, am, sa = _flat(x)
+        M = sa.numel()
     dev = a.device
     if b.device != dev or bias is not None and (bias.device != dev or bias.dtype is not dt or bias.shape != (N,)):
         raise RuntimeError("linear_int8: weight and bias must be on x's device, bias (N,) of x's type")
     if bias is not None:
         bias = bias.contiguous()
-    out = torch.empty((*x.codes.shape[:-1], N), dtype=dt, device=dev)
-    _call(_hip.lib().coda_linear_int8, a, _hip.dtype_code(dt), a.data_ptr(), am, sa.data_ptr(), sa.numel(), b.data_ptr(),
-          bm, sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
+    out = torch.empty((*shape[:-1], N), dtype=dt, device=dev)
+    _call(_hip.lib().coda_linear_int8, a, _hip.dtype_code(dt), a.data_ptr(), am, None if sa is None else sa.data_ptr(), M,
+          shape[-1], b.data_ptr(), bm, sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
     return out
 
 
@@ -298,20 +311,18 @@ class Int8Mixin:
             self.__dict__["_int8_made"] = (tag, val, _Made(*val[:5]))
         return val
 
-    def _int8_tokens(self, x) -> Int8Rows:
-        r = x if isinstance(x, Int8Rows) else quantize_rows(x)
-        if r.codes.dim() != 3 or r.cols != self.embed_dim:
-            raise RuntimeError(f"tokens {tuple(r.shape)} are not (B, L, {self.embed_dim})")
-        return r
-
     def _front_int8(self, x, p0: int, tables: Optional[tuple] = None):
         """q (B,H,L,Dh) before RoPE, k (B,Hkv,L,Dh) roped, v, the gate (B,L)
         float32 (None without one), lambda (B,H,L) and the RoPE tables of
         positions p0 .., of x (B,L,D), a tensor or Int8Rows.  tables: made by
         the launch or given, as (coda_proj_params or None, address of cos, of
         sin)."""
-        r = self._int8_tokens(x)
-        B, L, _ = r.shape
+        if len(x.shape) != 3 or x.shape[2] != self.embed_dim:
+            raise RuntimeError(f"tokens {tuple(x.shape)} are not (B, L, {self.embed_dim})")
+        r = x
+        B, L, D = r.shape
+        if not isinstance(x, Int8Rows) and B * L > FLOAT_ROWS:
+            r = quantize_rows(x)
         H, Hkv, Dh, dt, dev = self.num_heads, self.num_kv_heads, self.head_dim, r.dtype, r.device
         w, sw, bias = self._int8_weights()[:3]
         if w.device != dev:
@@ -323,7 +334,7 @@ class Int8Mixin:
         v = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
         lam = torch.empty((B, L, H), dtype=dt, device=dev)
         g = torch.empty((B, L), dtype=torch.float32, device=dev) if self._has_gate() else None
-        codes, sm, scales = _flat(r)
+        codes, sm, scales = _flat(r) if isinstance(r, Int8Rows) else (*_rows_of(r), None)
         d = self._proj_desc(r, B * L, L, cos, sin)
         params = None
         if tables is not None:
@@ -332,7 +343,7 @@ class Int8Mixin:
         d.x, d.x_sm = codes.data_ptr(), sm
         d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q.data_ptr(), Fq, k.data_ptr(), Fk, v.data_ptr(), Fk
         d.lam, d.lam_sm, d.g = lam.data_ptr(), H, _hip.ptr(g)
-        _call(_hip.lib().coda_project_int8, codes, d, scales.data_ptr(), sw.data_ptr(), w.stride(0), w.shape[1],
+        _call(_hip.lib().coda_project_int8, codes, d, _hip.ptr(scales), sw.data_ptr(), w.stride(0), w.shape[1],
               params)
         return (q.permute(0, 2, 1, 3), k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3), g, lam.permute(0, 2, 1), cos, sin)
 
@@ -341,4 +352,4 @@ class Int8Mixin:
         if not self.int8_projections:
             return self.o_proj(heads)
         w, sw, bias = self._int8_weights()[3:]
-        return linear_int8(quantize_rows(heads), _made(w, sw, heads.shape[-1], heads.dtype), bias)
+        return linear_int8(heads, _made(w, sw, heads.shape[-1], heads.dtype), bias)

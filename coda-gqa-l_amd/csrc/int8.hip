@@ -63,6 +63,45 @@ __device__ __forceinline__ void run_st(T* p, int n, const Run8<T>& r) {
   }
 }
 
+// Codes of a row whose largest magnitude is P: code(p) = rint(127 p / P), the
+// quotient to the last bit: n = 127 p, times the reciprocal, then its
+// remainder's share.  In fp32 P is brought to [1, 2) (p by the same power of
+// two), where neither leaves the range.
+template <typename R>
+struct Coder {
+  // leaves a quotient's nearest integer (ties to even) in its low bits: 1.5
+  // times 2^23 or 2^52
+  static constexpr R kShift = sizeof(R) == 4 ? (R)12582912. : (R)6755399441055744.;
+  R k, Q, inv;
+  __device__ __forceinline__ Coder(double P, bool fine) : k(127), Q((R)P), inv(0) {
+    if (!fine) return;
+    if constexpr (sizeof(R) == 4) {
+      int ex;
+      Q = (float)(2. * frexp(P, &ex));
+      k = (float)ldexp(127., min(1 - ex, 119));
+      Q = (float)ldexp((double)Q, min(1 - ex, 119) - (1 - ex));
+    }
+    inv = (R)1 / Q;
+  }
+  __device__ __forceinline__ uint32_t operator()(R p) const {  // in the low byte
+    const R n = p * k, q0 = n * inv;
+    const R q = __builtin_elementwise_fma(__builtin_elementwise_fma(-q0, Q, n), inv, q0) + kShift;
+    if constexpr (sizeof(R) == 4) return __builtin_bit_cast(uint32_t, q);
+    else return (uint32_t)__builtin_bit_cast(uint64_t, q);
+  }
+};
+// the low bytes of eight
+__device__ __forceinline__ uint2 pack8(const uint32_t (&c)[8]) {
+  const auto four = [](uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(e, d, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                                 0x05040100u);
+  };
+  return uint2{four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7])};
+}
+// the type that p and P of plain rows need
+template <typename T>
+using PlainR = typename std::conditional<sizeof(T) == 2, float, double>::type;
+
 // Rows in 8 bits, with p_i = x_i (plain) or p_i = s_i w_i (norm; s = x +
 // residual, rounded to T and written):
 //   P = max |p|, code_i = rint(127 p_i / P),
@@ -83,10 +122,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void codes_kernel(
     int D, float eps, T* __restrict__ sum_out, int64_t s_sm, int8_t* __restrict__ codes, int64_t c_sm,
     float* __restrict__ scales) {
   using E = Elt<T>;
-  // the type of p and of the quotient, and the shift that leaves a quotient's
-  // nearest integer (ties to even) in its low bits: 1.5 times 2^23 or 2^52
-  typedef typename std::conditional<!NORM && sizeof(T) == 2, float, double>::type R;
-  constexpr R kShift = sizeof(R) == 4 ? (R)12582912. : (R)6755399441055744.;
+  typedef typename std::conditional<NORM, double, PlainR<T>>::type R;
   constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -152,19 +188,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void codes_kernel(
     if constexpr (NORM) sc /= sqrt(ss / (double)D + (double)eps);
     scales[row] = ss != ss ? __builtin_nanf("") : P > 0. ? (float)sc : 0.f;
   }
-  // 127 p / P to the last bit: n = 127 p, the quotient by the reciprocal, then
-  // its remainder's share.  In fp32 P is brought to [1, 2) (p by the same
-  // power of two), where neither leaves the range.
-  R k = 127, Q = (R)P, inv = 0;
-  if (fine) {
-    if constexpr (sizeof(R) == 4) {
-      int ex;
-      Q = (float)(2. * frexp(P, &ex));
-      k = (float)ldexp(127., min(1 - ex, 119));
-      Q = (float)ldexp((double)Q, min(1 - ex, 119) - (1 - ex));
-    }
-    inv = (R)1 / Q;
-  }
+  const Coder<R> code(P, fine);
   int8_t* cr = codes + row * c_sm;
   // (the row's tail: zeros up to a whole 128 bytes)
   const int padded = (D + kPad - 1) / kPad * kPad;
@@ -174,21 +198,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void codes_kernel(
     if (at >= padded) continue;
     uint32_t c[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const R n = p[i * 8 + e] * k, q0 = n * inv;
-      const R q = __builtin_elementwise_fma(__builtin_elementwise_fma(-q0, Q, n), inv, q0) + kShift;
-      if constexpr (sizeof(R) == 4) c[e] = __builtin_bit_cast(uint32_t, q);
-      else c[e] = (uint32_t)__builtin_bit_cast(uint64_t, q);
-    }
-    uint2 v{0u, 0u};
-    if (fine) {
-      // the low bytes of four
-      const auto four = [](uint32_t a, uint32_t b, uint32_t cc, uint32_t d) {
-        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, cc, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
-                                     0x05040100u);
-      };
-      v = uint2{four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7])};
-    }
+    for (int e = 0; e < 8; ++e) c[e] = code(p[i * 8 + e]);
+    const uint2 v = fine ? pack8(c) : uint2{0u, 0u};
     *reinterpret_cast<uint2*>(cr + at) = v;
   }
 }
@@ -331,17 +342,18 @@ struct FastDiv {
 // The projection front end: the sections and roundings of FrontEpilogue (a
 // value is rounded to T before the RoPE or the sigmoid), with all that does
 // not change from token to token found once.  TABLES: angles that the launch
-// makes itself where tab says so.
-template <typename T, bool TABLES>
+// makes itself where tab says so.  N: features of a run: 8 where heads and
+// rows allow 16-byte pieces, else 4.
+template <typename T, bool TABLES, int N>
 struct FrontSink {
   typedef T Out;
   typedef Elt<T> E;
-  static constexpr int kRun = 4;
+  static constexpr int kRun = N;
   coda_proj_desc d;
   FrontTables tab;
   FastDiv len;  // of a sequence: table row = token % L
   int n_feat;
-  // Where four features go: q or v (kind 0), k (1), single lambdas / gates
+  // Where a run of features goes: q or v (kind 0), k (1), single lambdas / gates
   // (2); at: of a token 0's first channel (kind 1: of its head), c: that
   // channel (kind 2: the feature)
   struct Lane {
@@ -360,48 +372,59 @@ struct FrontSink {
     if (f < Fq + 2 * Fk) return Lane{0, 0, (T*)d.v + (f - Fq - Fk), d.v_sm};
     return Lane{2, f, nullptr, 0};
   }
-  template <int R>
-  __device__ __forceinline__ void put(const Lane& l, int m, int step, int rows, const Feats<T, 4> (&v)[R]) const {
-    // (8-byte rows: see the entry's checks)
-    typedef uint32_t V __attribute__((ext_vector_type(sizeof(T)), aligned(8)));  // four T
-    struct alignas(2 * sizeof(T)) Two {
-      T v[2];
-    };
+  // a row's runs of n T's: at 8-byte addresses at least (the entry's checks)
+  template <int n>
+  static __device__ __forceinline__ void st(T* p, const Feats<T, n>& v) {
+    typedef uint32_t V __attribute__((ext_vector_type(sizeof(v) / 4), aligned(sizeof(v) == 4 ? 4 : 8)));
+    *reinterpret_cast<V*>(p) = __builtin_bit_cast(V, v);
+  }
+  template <int M, int R>
+  __device__ __forceinline__ void put(const Lane& l, int m, int step, int rows, const Feats<T, M> (&v)[R]) const {
     T* row = l.at + (int64_t)m * l.sm;
     const int64_t next = step * l.sm;
     if (l.kind == 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (m + r * step < rows) *reinterpret_cast<V*>(row + r * next) = __builtin_bit_cast(V, v[r]);
+        if (m + r * step < rows) st(row + r * next, v[r]);
     } else if (l.kind == 1) {
+      typedef Feats<T, M / 2> Half;  // a table's entries of M / 2 pairs, at any element address
+      struct Any {
+        T v[M / 2];
+      };
       const int half = d.Dh / 2, p = l.c / 2;
       const bool inter = d.rope_interleaved != 0;
-      float2 a[R][2];
+      Any cs[R], sn[R];
+      int prow[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int prow = (int)len.mod((uint32_t)min(m + r * step, rows - 1));
-        const T* cs = (const T*)d.rope_cos + (int64_t)prow * half + p;
-        const T* sn = (const T*)d.rope_sin + (int64_t)prow * half + p;
-#pragma unroll
-        for (int pp = 0; pp < 2; ++pp)
-          a[r][pp] = TABLES && tab.inv_freq ? rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + prow, p + pp)
-                                            : float2{E::ld(cs[pp]), E::ld(sn[pp])};
+        prow[r] = (int)len.mod((uint32_t)min(m + r * step, rows - 1));
+        if (!(TABLES && tab.inv_freq)) {
+          typedef uint16_t U __attribute__((ext_vector_type(sizeof(Any) / 2), aligned(2)));
+          const int64_t at = (int64_t)prow[r] * half + p;
+          cs[r] = __builtin_bit_cast(Any, *reinterpret_cast<const U*>((const T*)d.rope_cos + at));
+          sn[r] = __builtin_bit_cast(Any, *reinterpret_cast<const U*>((const T*)d.rope_sin + at));
+        }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (m + r * step >= rows) continue;
-        float o[4];
+        Feats<T, M> o;  // pair by pair
+        Half first, second;
 #pragma unroll
-        for (int pp = 0; pp < 2; ++pp)
-          rope_pair_t<T>(E::ld(v[r].v[2 * pp]), E::ld(v[r].v[2 * pp + 1]), a[r][pp].x, a[r][pp].y, inter, o[2 * pp],
-                         o[2 * pp + 1]);
+        for (int pp = 0; pp < M / 2; ++pp) {
+          const float2 a = TABLES && tab.inv_freq ? rope_angle<T>(tab.inv_freq, tab.inv_dtype, tab.p0 + prow[r], p + pp)
+                                                  : float2{E::ld(cs[r].v[pp]), E::ld(sn[r].v[pp])};
+          float o0, o1;
+          rope_pair_t<T>(E::ld(v[r].v[2 * pp]), E::ld(v[r].v[2 * pp + 1]), a.x, a.y, inter, o0, o1);
+          o.v[2 * pp] = first.v[pp] = E::st(o0);
+          o.v[2 * pp + 1] = second.v[pp] = E::st(o1);
+        }
         T* at = row + r * next;
         if (inter) {
-          const Feats<T, 4> w{{E::st(o[0]), E::st(o[1]), E::st(o[2]), E::st(o[3])}};
-          *reinterpret_cast<V*>(at + l.c) = __builtin_bit_cast(V, w);
-        } else {  // pairs (p, p + half): channels p, p + 1 and the same + half
-          *reinterpret_cast<Two*>(at + p) = Two{{E::st(o[0]), E::st(o[2])}};
-          *reinterpret_cast<Two*>(at + p + half) = Two{{E::st(o[1]), E::st(o[3])}};
+          st(at + l.c, o);
+        } else {  // pairs (p, p + half): channels p .. and the same + half
+          st(at + p, first);
+          st(at + p + half, second);
         }
       }
     } else {
@@ -409,7 +432,7 @@ struct FrontSink {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < M; ++e) {
           const int f = l.c + e;
           const int64_t mr = m + r * step;
           if (f >= n_feat || mr >= rows) continue;
@@ -727,6 +750,112 @@ struct RowsSink {
   __device__ __forceinline__ void once(int t) const { sink.once(t); }
 };
 
+static constexpr int kFloatRows = 4;
+// Up to 4 tokens as they come, quantised by every workgroup while its first
+// weights are on their way: the codes and scales of codes_kernel, the sums of
+// proj_rows.  The codes lie in LDS, rows of K + 16 bytes; two waves or more
+// share a row, which they read twice (the second time from cache).  K: of the
+// weights, D <= K.  One launch against two, us, bf16: 4096 x 6177 10.1 and
+// 11.3 at 1 row, 11.3 and 11.6 at 4, 13.8 and 12.0 at 8; 4096 x 4096 7.3 and
+// 8.8, 512 x 649 4.1 and 4.9 at 1 row.
+template <typename T, int RB, typename Sink>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void int8_rows_of(
+    const T* __restrict__ X, int64_t x_sm, int M, int D, const Int8Mat W, int K, const Sink sink) {
+  using E = Elt<T>;
+  typedef PlainR<T> R;
+  extern __shared__ __attribute__((aligned(16))) char rows_smem[];
+  __shared__ double tops[8];
+  __shared__ float scales[kFloatRows];
+  constexpr int LP = 4;  // pairs of k-steps in flight ahead of the products
+  const int f0 = blockIdx.x * 16 * RB;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), r16 = lane & 15, kq = lane >> 4;
+  const int pairs = K / 128, p0 = pairs * wv / 8, np = pairs * (wv + 1) / 8 - p0;
+  const int8_t* wr[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) wr[i] = W.p + (int64_t)min(f0 + 16 * i + r16, W.rows - 1) * W.sm + 128 * p0 + 16 * kq;
+  pu32x4 a[LP][RB][2];
+  auto load = [&](int u, int p) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) a[u][i][h] = *reinterpret_cast<const pu32x4*>(wr[i] + 128 * p + 64 * h);
+  };
+#pragma unroll
+  for (int u = 0; u < LP; ++u)
+    if (u < np) load(u, u);
+  const int share = M == 1 ? 8 : M == 2 ? 4 : 2, step = 512 * share;  // waves a row; elements a turn
+  const int m = wv / share, first = (wv % share * 64 + lane) * 8;
+  const T* xr = X + (int64_t)min(m, M - 1) * x_sm;
+  R top = 0, bad = 0;
+  for (int k = first; k < D; k += step) {
+    const Run8<T> v = run_ld(xr + k, D - k);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const R p = (R)E::ld(v.v[e]);
+      top = __builtin_elementwise_max(top, __builtin_elementwise_abs(p));
+      bad = __builtin_elementwise_fma(p, (R)0, bad);
+    }
+  }
+  double P = wave_reduce((double)top, true) + wave_reduce((double)bad, false);  // NaN: no number in the row
+  if (lane == 0) tops[wv] = P;
+  __syncthreads();
+  P = tops[m * share];
+  for (int i = 1; i < share; ++i) {
+    const double o = tops[m * share + i];
+    P = P != P || o != o ? P + o : fmax(P, o);
+  }
+  const bool fine = P == P && P > 0.;
+  if (m < M) {
+    if (lane == 0) scales[m] = fine || P != P ? (float)(P / 127.) : 0.f;
+    const Coder<R> code(P, fine);
+    for (int k = first; k < K; k += step) {
+      const Run8<T> v = run_ld(xr + k, D - k);
+      uint32_t c[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = code((R)E::ld(v.v[e]));
+      *reinterpret_cast<uint2*>(rows_smem + m * (K + 16) + k) = fine ? pack8(c) : uint2{0u, 0u};
+    }
+  }
+  __syncthreads();
+  i32x4 acc[RB][1];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) acc[i][0] = i32x4{0, 0, 0, 0};
+  const char* br = rows_smem + min(r16, M - 1) * (K + 16) + 128 * p0 + 16 * kq;
+  for (int p = 0; p < np; p += LP)
+#pragma unroll
+    for (int u = 0; u < LP; ++u) {
+      if (p + u >= np) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const pu32x4 b = *reinterpret_cast<const pu32x4*>(br + 128 * (p + u) + 64 * h);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) acc[i][0] = rows_mfma<int8_t>(a[u][i][h], b, acc[i][0]);
+      }
+      if (p + u + LP < np) load(u, p + u + LP);
+    }
+  __syncthreads();
+  rows_finish<1, RB>(acc, rows_smem, W.rows, M, 0, RowsSink<Sink>{sink, scales, W.scales, W.rows});
+}
+template <typename T, int RB, typename Sink>
+static int launch_rows_of(const T* X, int64_t x_sm, int M, int D, const Int8Mat& W, int K, const Sink& sink,
+                          hipStream_t st, const char* who) {
+  const size_t codes = (size_t)M * (K + 16), lds = codes > RowsLds<1, RB>::kBytes ? codes : RowsLds<1, RB>::kBytes;
+  const int rc = lds_limit<int8_rows_of<T, RB, Sink>>(lds, who);
+  if (rc) return rc;
+  hipLaunchKernelGGL((int8_rows_of<T, RB, Sink>), dim3((W.rows + 16 * RB - 1) / (16 * RB)), dim3(512), lds, st, X, x_sm, M,
+                     D, W, K, sink);
+  return check_launch("int8_rows_of");
+}
+template <typename T, typename Sink>
+static int launch_of(const void* x, int64_t x_sm, int M, int D, const Int8Mat& W, int K, const Sink& sink,
+                     hipStream_t st, const char* who) {
+  switch (rows_rb(W.rows)) {
+    case 1: return launch_rows_of<T, 1>((const T*)x, x_sm, M, D, W, K, sink, st, who);
+    case 2: return launch_rows_of<T, 2>((const T*)x, x_sm, M, D, W, K, sink, st, who);
+    default: return launch_rows_of<T, 3>((const T*)x, x_sm, M, D, W, K, sink, st, who);
+  }
+}
+
 static constexpr int kFewRows = 128;
 template <typename Sink>
 static int launch_few(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
@@ -754,15 +883,22 @@ static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scale
 }
 static bool int8_dtype(int t) { return t == CODA_F32 || t == CODA_BF16 || t == CODA_F16; }
 
-// The two operands of a product
-static int check_mats(const Int8Mat& X, const Int8Mat& W, int K, const char* who) {
+// The two operands of a product: of X codes, or (no scales) D elements a row
+static int check_mats(const Int8Mat& X, int D, const Int8Mat& W, int K, const char* who) {
   CODA_REQUIRE(X.rows >= 0 && W.rows > 0 && K > 0 && K % kPad == 0 && K <= kMaxK,
                "%s: bad sizes rows=%d features=%d K=%d (K a multiple of %d, at most %d: int32 holds the sum)", who, X.rows,
                W.rows, K, kPad, kMaxK);
-  CODA_REQUIRE(W.p && W.scales && (X.rows == 0 || (X.p && X.scales)), "%s: null pointer", who);
-  CODA_REQUIRE((uintptr_t)X.p % 16 == 0 && (uintptr_t)W.p % 16 == 0 && X.sm % 16 == 0 && W.sm % 16 == 0 &&
-                   X.sm >= 0 && W.sm >= 0,
-               "%s: rows of codes must lie at 16-byte addresses", who);
+  CODA_REQUIRE(W.p && W.scales && (X.rows == 0 || X.p), "%s: null pointer", who);
+  CODA_REQUIRE((uintptr_t)W.p % 16 == 0 && W.sm % 16 == 0 && W.sm >= 0, "%s: rows of codes must lie at 16-byte addresses",
+               who);
+  if (X.scales || X.rows == 0) {
+    CODA_REQUIRE((uintptr_t)X.p % 16 == 0 && X.sm % 16 == 0 && X.sm >= 0, "%s: rows of codes must lie at 16-byte addresses",
+                 who);
+  } else {
+    CODA_REQUIRE(X.rows <= kFloatRows, "%s: %d token rows without scales (at most %d are quantised by the launch)", who,
+                 X.rows, kFloatRows);
+    CODA_REQUIRE(D > 0 && D <= K && X.sm >= 0, "%s: rows of %d elements for K=%d", who, D, K);
+  }
   return CODA_OK;
 }
 
@@ -815,21 +951,24 @@ extern "C" int coda_dequantize_rows(int dtype, const int8_t* codes, int64_t c_sm
 #undef RUN
 }
 
-extern "C" int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const float* x_scales, int M, const int8_t* w,
-                                int64_t w_sm, const float* w_scales, int n_feat, int K, const void* bias, void* out,
-                                int64_t o_sm, void* stream) {
+extern "C" int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const float* x_scales, int M, int D,
+                                const int8_t* w, int64_t w_sm, const float* w_scales, int n_feat, int K, const void* bias,
+                                void* out, int64_t o_sm, void* stream) {
   const char* who = "coda_linear_int8";
   CODA_REQUIRE(int8_dtype(dtype), "%s: dtype must be CODA_F32, CODA_BF16 or CODA_F16", who);
-  const Int8Mat X{x, x_sm, x_scales, M}, W{w, w_sm, w_scales, n_feat};
-  const int rc = check_mats(X, W, K, who);
+  const Int8Mat X{(const int8_t*)x, x_sm, x_scales, M}, W{w, w_sm, w_scales, n_feat};
+  const int rc = check_mats(X, D, W, K, who);
   if (rc || M == 0) return rc;
   CODA_REQUIRE(out && o_sm >= n_feat, "%s: no output, or its rows shorter than %d features", who, n_feat);
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T)                                                              \
-  (M <= kFewRows ? launch_few(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who) \
-                 : launch_many(X, W, K, LinearSink<T>{(T*)out, (const T*)bias, o_sm, n_feat}, st, who))
-  return dtype == CODA_F32 ? RUN(float) : dtype == CODA_BF16 ? RUN(bf16_t) : RUN(f16_t);
-#undef RUN
+  const auto run = [&](auto t) {
+    typedef decltype(t) T;
+    const LinearSink<T> sink{(T*)out, (const T*)bias, o_sm, n_feat};
+    return !x_scales       ? launch_of<T>(x, x_sm, M, D, W, K, sink, st, who)
+           : M <= kFewRows ? launch_few(X, W, K, sink, st, who)
+                           : launch_many(X, W, K, sink, st, who);
+  };
+  return dtype == CODA_F32 ? run(float{}) : dtype == CODA_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
 
 extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales, const float* w_scales, int64_t w_sm,
@@ -841,7 +980,7 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
                "%s: bad sizes M=%d H=%d Hkv=%d Dh=%d L=%d", who, d->M, d->H, d->Hkv, d->Dh, d->L);
   const int n_feat = d->H * d->Dh + 2 * d->Hkv * d->Dh + d->H + (d->gate ? 1 : 0);
   const Int8Mat X{(const int8_t*)d->x, d->x_sm, x_scales, d->M}, W{(const int8_t*)d->w, w_sm, w_scales, n_feat};
-  const int rc = check_mats(X, W, K, who);
+  const int rc = check_mats(X, d->D, W, K, who);
   if (rc || d->M == 0) return rc;
   const bool own = p && p->inv_freq;
   CODA_REQUIRE(d->bias && (own || (d->rope_cos && d->rope_sin)) && d->q && d->k && d->v && d->lam && (d->g || !d->gate),
@@ -863,9 +1002,15 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
   }
   const hipStream_t st = (hipStream_t)stream;
   const FastDiv len(d->L);
-#define RUN(T)                                                                        \
-  (d->M <= kFewRows ? launch_few(X, W, K, FrontSink<T, true>{*d, tab, len, n_feat}, st, who) \
-                    : launch_many(X, W, K, FrontSink<T, false>{*d, tab, len, n_feat}, st, who))
-  return d->dtype == CODA_BF16 ? RUN(bf16_t) : RUN(float);
-#undef RUN
+  const auto run = [&](auto t) {
+    typedef decltype(t) T;
+    if (d->M <= kFewRows) {
+      const FrontSink<T, true, 4> sink{*d, tab, len, n_feat};
+      return x_scales ? launch_few(X, W, K, sink, st, who) : launch_of<T>(d->x, d->x_sm, d->M, d->D, W, K, sink, st, who);
+    }
+    if constexpr (sizeof(T) == 2)
+      if (d->Dh % 8 == 0) return launch_many(X, W, K, FrontSink<T, false, 8>{*d, tab, len, n_feat}, st, who);
+    return launch_many(X, W, K, FrontSink<T, false, 4>{*d, tab, len, n_feat}, st, who);
+  };
+  return d->dtype == CODA_BF16 ? run(bf16_t{}) : run(float{});
 }

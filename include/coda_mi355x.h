@@ -214,16 +214,20 @@ int coda_dequantize_rows(int dtype, const int8_t* codes, int64_t c_sm, const flo
                          int64_t o_sm, void* stream);
 
 /* out[m, f] = (sum_k x[m, k] w[f, k]) x_scales[m] w_scales[f] + bias[f], the
- * sum exact in int32, one rounding to dtype.  K: the padded length, a
- * multiple of 128 and at most 130944; bias (n_feat) of dtype, or NULL. */
-int coda_linear_int8(int dtype, const int8_t* x, int64_t x_sm, const float* x_scales, int M, const int8_t* w,
+ * sum exact in int32, one rounding to dtype.  x codes (x_sm bytes from row to
+ * row; D unused), or, x_scales NULL and M at most 4, rows of D elements of
+ * dtype that the launch quantises as coda_quantize_rows does (x_sm
+ * elements).  K: the weights' padded length, a multiple of 128 and at most
+ * 130944; bias (n_feat) of dtype, or NULL. */
+int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const float* x_scales, int M, int D, const int8_t* w,
                      int64_t w_sm, const float* w_scales, int n_feat, int K, const void* bias, void* out, int64_t o_sm,
                      void* stream);
 
 /* The projection front end (coda_project) on rows in 8 bits, for any number
- * of token rows: d->x (M, K) and d->w (n_feat, K) are codes (d->x_sm and w_sm
- * in bytes, w row-major in coda_project's row order; D and w_layout unused),
- * dtype CODA_BF16 or CODA_F32 the type of q, k, v, lam and the tables.
+ * of token rows: d->w (n_feat, K) is codes (w_sm bytes from row to row,
+ * row-major in coda_project's row order; w_layout unused), d->x codes, or
+ * with x_scales NULL rows of d->D elements, as in coda_linear_int8; dtype
+ * CODA_BF16 or CODA_F32 the type of q, k, v, lam and the tables.
  * gate == 0 leaves g alone (it may be NULL).  p may be NULL; of it only the
  * tables are read, as in coda_project_params (at most 128 token rows then). */
 int coda_project_int8(const coda_proj_desc* d, const float* x_scales, const float* w_scales, int64_t w_sm, int K,

@@ -37,7 +37,7 @@ def test_no_host_path():
     x = torch.zeros(2, 128)
     r = Int8Rows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), 128, torch.float32)
     for call in (lambda: coda_gqa_l.quantize_rows(x), lambda: coda_gqa_l.rms_norm_int8(x, x[0]),
-                 lambda: coda_gqa_l.linear_int8(r, r), r.dequantize):
+                 lambda: coda_gqa_l.linear_int8(r, r), lambda: coda_gqa_l.linear_int8(x, r), r.dequantize):
         with pytest.raises(RuntimeError, match="HIP devices only"):
             call()
 
@@ -84,10 +84,11 @@ def test_rms_norm_entry(change, error):
     (dict(K=64), "multiple of 128"), (dict(K=131072), "int32"), (dict(K=0), "sizes"), (dict(n_feat=0), "sizes"),
     (dict(M=-1), "sizes"), (dict(x=P + 1), "16-byte"), (dict(w_sm=130), "16-byte"), (dict(w=None), "null"),
     (dict(x=None), "null"), (dict(out=None), "output"), (dict(o_sm=9), "output"), (dict(dtype=3), "dtype"),
-    (dict(x_sm=-128), "16-byte"),
+    (dict(x_sm=-128), "16-byte"), (dict(x_scales=None, M=5), "at most 4"), (dict(x_scales=None, D=129), "129 elements"),
+    (dict(x_scales=None, D=0), "0 elements"), (dict(x_scales=None, x=None), "null"),
 ])
 def test_linear_entry(change, error):
-    a = dict(dtype=1, x=P, x_sm=128, x_scales=P, M=3, w=P, w_sm=128, w_scales=P, n_feat=10, K=128, bias=None, out=P,
+    a = dict(dtype=1, x=P, x_sm=128, x_scales=P, M=3, D=128, w=P, w_sm=128, w_scales=P, n_feat=10, K=128, bias=None, out=P,
              o_sm=10)
     a.update(change)
     L = _hip.lib()

@@ -258,12 +258,34 @@ def test_writes_nothing_else(M):
     (a, sa), (b, sb) = _int8(g, M, K), _int8(g, N, K)
     for code, dt in enumerate((torch.float32, torch.bfloat16, torch.float16)):
         out = torch.full((M + 2, N + 5), 7.0, dtype=dt, device=DEV)
-        _hip.check(_hip.lib().coda_linear_int8(code, a.data_ptr(), K, sa.data_ptr(), M, b.data_ptr(), K, sb.data_ptr(), N,
+        _hip.check(_hip.lib().coda_linear_int8(code, a.data_ptr(), K, sa.data_ptr(), M, 0, b.data_ptr(), K, sb.data_ptr(), N,
                                                K, None, out[1, 2:].data_ptr(), N + 5, _hip.stream_of(a)))
         want = linear_int8(Int8Rows(a, sa, K, dt), Int8Rows(b, sb, K, dt))
         assert torch.equal(out[1:-1, 2:2 + N], want)
         out[1:-1, 2:2 + N] = 7.0
         assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 4096, 6177), (2, 100, 7), (3, 127, 50), (5, 1000, 515), (16, 8192, 130),
+                                   (16, 333, 2049), (17, 512, 64), (150, 200, 300), (1, 130, 8200), (4, 30001, 33)])
+def test_tokens_as_they_come(M, K, N, dtype):
+    """A float x: the bits of quantize_rows and the product of its rows, rows
+    without a number among them."""
+    g = _gen(M * K + N)
+    x, q = _rand(g, M, K, dtype=dtype), quantize_rows(_rand(g, N, K, dtype=dtype))
+    if M > 2:
+        x[1], x[2, K // 2] = 0, float("inf")
+    bias = _rand(g, N, dtype=dtype)
+    for b in (None, bias):
+        assert torch.equal(linear_int8(x, q, b).nan_to_num(7.0), linear_int8(quantize_rows(x), q, b).nan_to_num(7.0))
+    if M > 2:
+        y = linear_int8(x, q)
+        assert not y[1].any() and y[2].isnan().all()
+    wide = torch.full((M, K + 3), float("nan"), device=DEV, dtype=dtype)[:, 2:K + 2].copy_(x)
+    for v in (wide, x.t().contiguous().t(), x.view(1, M, 1, K)):
+        assert torch.equal(linear_int8(v, q).reshape(M, N).nan_to_num(7.0), linear_int8(x, q).nan_to_num(7.0))
+    assert torch.equal(linear_int8(x[:1].expand(M, K), q), linear_int8(x[:1], q).expand(M, N))
 
 
 # ---------------------------------------------------------------- together
@@ -353,7 +375,7 @@ def test_refusals_on_the_device():
         quantize_rows(x.double())
     q = quantize_rows(x)
     with pytest.raises(TypeError, match="Int8Rows"):
-        linear_int8(x, q)
+        linear_int8(q, x)
     with pytest.raises(RuntimeError, match="does not fit"):
         linear_int8(q, quantize_rows(x[:, :63]))
     with pytest.raises(RuntimeError, match="bias"):

@@ -71,7 +71,8 @@ def _out(m, heads):
 @pytest.mark.parametrize("B,L,D,H,Hkv,inter,gate", [
     (1, 1, 512, 8, 2, True, True), (5, 1, 512, 8, 2, False, True), (33, 1, 320, 10, 5, True, False),
     (128, 1, 256, 4, 1, False, True), (2, 100, 512, 4, 4, True, True), (3, 77, 320, 5, 1, False, True),
-    (1, 999, 768, 12, 4, False, False), (2, 4097, 256, 4, 2, True, True), (4, 4100, 768, 6, 3, False, True),
+    (1, 999, 768, 12, 4, False, False), (2, 300, 240, 20, 4, True, False), (3, 150, 240, 20, 5, False, False),
+    (2, 2, 240, 20, 4, False, False), (2, 4097, 256, 4, 2, True, True), (4, 4100, 768, 6, 3, False, True),
 ])
 @torch.no_grad()
 def test_front(B, L, D, H, Hkv, inter, gate, dtype):
