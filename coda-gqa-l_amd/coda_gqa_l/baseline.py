@@ -86,9 +86,8 @@ class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
         H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
         int8 = self._int8_on(x)
         if past_key_value is not None and self._decode_ok(x, past_key_value, is_causal):
-            if int8:
-                return self._decode_int8(x, *past_key_value)
-            rows = self._front_rows(x)
+            # (a launch makes the tables of up to 128 rows)
+            rows = self._front_rows(x) if not int8 else () if B * L <= 128 else None
             if rows is not None:
                 return self._decode(x, rows, *past_key_value)
         if int8:
@@ -132,17 +131,17 @@ class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
                 not (k.data_ptr() % 16 or v.data_ptr() % 16) and k.device == v.device == x.device and
                 not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)))
 
-    def _decode(self, x: torch.Tensor, rows: tuple, k_past: torch.Tensor, v_past: torch.Tensor):
+    def _decode(self, x, rows: tuple, k_past: torch.Tensor, v_past: torch.Tensor):
         """forward() on top of a past for a few new tokens: one launch for the
-        projections, the RoPE of k and the angle tables (coda_project_params),
-        one for the attention and the concatenated K / V (coda_attn_append,
-        which reads the past once for both), the merge of its splits, and
-        o_proj; all on the parameters as they stand at the call."""
+        projections, the RoPE of k and the angle tables (coda_project_params,
+        or without rows coda_project_int8), one for the attention and the
+        concatenated K / V (coda_attn_append, which reads the past once for
+        both), the merge of its splits, and o_proj; all on the parameters as
+        they stand at the call."""
         B, L, D = x.shape
         H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
-        past, M, e, half = k_past.shape[2], B * L, x.element_size(), Dh // 2
-        lib, stream, dev = _hip.lib(), _hip.stream_of(x), x.device
-        xs = _aligned(x)
+        past, M, e, half = k_past.shape[2], B * L, x.dtype.itemsize, Dh // 2
+        lib, stream, dev = _hip.lib(), _hip.stream_of(k_past), x.device
         # q | k | v | lambda | gate of the new tokens, RoPE cos | sin, theta
         # cos | sin in one buffer
         sizes = [M * D * e, M * Hkv * Dh * e, M * Hkv * Dh * e, M * H * e, M * 4, L * half * e, L * half * e,
@@ -156,28 +155,17 @@ class CoDAGQA(Int8Mixin, RowsMixin, nn.Module):
         (rc_p, rs_p, tc_p, ts_p), keep = self._launch_tables(p, x, past, (rc_p, rs_p, tc_p, ts_p))
         d = self._proj_desc(x, M, L)
         d.rope_cos, d.rope_sin = rc_p, rs_p
-        d.x, d.x_sm = xs.data_ptr(), D
         d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q_p, D, k_p, Hkv * Dh, v_p, Hkv * Dh
         d.lam, d.lam_sm, d.g = l_p, H, g_p
-        _hip.check(lib.coda_project_params(d, p, stream))
-        heads, kv = self._append(x, (q_p, k_p, v_p, l_p, rc_p, rs_p, tc_p, ts_p), k_past, v_past)
-        return self._out_rows(heads), kv
-
-    def _decode_int8(self, x, k_past: torch.Tensor, v_past: torch.Tensor):
-        """_decode with 8-bit projections."""
-        B, L, _ = x.shape
-        past, half, p = k_past.shape[2], self.head_dim // 2, None
-        tables = tuple(torch.empty((n, half), dtype=x.dtype, device=x.device)
-                       for n in (L, L, self.num_heads, self.num_heads))
-        if B * L <= 128:  # (as many rows as a launch makes tables for)
-            p = _hip.ProjParams()
-            at, keep = self._launch_tables(p, x, past, tuple(t.data_ptr() for t in tables))
+        if rows:
+            xs = _aligned(x)
+            d.x, d.x_sm = xs.data_ptr(), D
+            _hip.check(lib.coda_project_params(d, p, stream))
         else:
-            tables = (*self._rope_tables(past, L, x.device, x.dtype), *self._theta_pair(x.dtype))
-            at = tuple(t.data_ptr() for t in tables)
-        q, k, v, _, lam, _, _ = self._front_int8(x, past, (p, *at[:2]))
-        heads, kv = self._append(x, (*(t.data_ptr() for t in (q, k, v, lam)), *at), k_past, v_past)
-        return self._out_proj(heads), kv
+            weights = self._int8_weights()
+            xs = self._launch_int8(x, d, weights, p)
+        heads, kv = self._append(x, (q_p, k_p, v_p, l_p, rc_p, rs_p, tc_p, ts_p), k_past, v_past)
+        return self._out_rows(heads) if rows else self._out_proj(heads, weights), kv
 
     def _launch_tables(self, p, x, p0: int, at: tuple):
         """Has the projection's launch make, at these addresses, the RoPE

@@ -311,45 +311,45 @@ class Int8Mixin:
             self.__dict__["_int8_made"] = (tag, val, _Made(*val[:5]))
         return val
 
-    def _front_int8(self, x, p0: int, tables: Optional[tuple] = None):
-        """q (B,H,L,Dh) before RoPE, k (B,Hkv,L,Dh) roped, v, the gate (B,L)
-        float32 (None without one), lambda (B,H,L) and the RoPE tables of
-        positions p0 .., of x (B,L,D), a tensor or Int8Rows.  tables: made by
-        the launch or given, as (coda_proj_params or None, address of cos, of
-        sin)."""
+    def _launch_int8(self, x, d, weights: tuple, p=None):
+        """The front end's product of x (B, L, D), a tensor or Int8Rows, into
+        d's outputs (coda_project_int8); what has to live until it has been
+        enqueued."""
         if len(x.shape) != 3 or x.shape[2] != self.embed_dim:
             raise RuntimeError(f"tokens {tuple(x.shape)} are not (B, L, {self.embed_dim})")
-        r = x
-        B, L, D = r.shape
-        if not isinstance(x, Int8Rows) and B * L > FLOAT_ROWS:
-            r = quantize_rows(x)
-        H, Hkv, Dh, dt, dev = self.num_heads, self.num_kv_heads, self.head_dim, r.dtype, r.device
-        w, sw, bias = self._int8_weights()[:3]
-        if w.device != dev:
-            raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
-        cos, sin = self._rope_tables(p0, L, dev, dt) if tables is None else (None, None)
+        w, sw, bias = weights[:3]
+        if w.device != x.device:
+            raise RuntimeError(f"projection weights on {w.device}, input on {x.device}")
+        if not isinstance(x, Int8Rows) and x.shape[0] * x.shape[1] > FLOAT_ROWS:
+            x = quantize_rows(x)
+        xs, d.x_sm, scales = _flat(x) if isinstance(x, Int8Rows) else (*_rows_of(x), None)
+        d.x, d.w, d.bias = xs.data_ptr(), w.data_ptr(), bias.data_ptr()
+        _call(_hip.lib().coda_project_int8, xs, d, _hip.ptr(scales), sw.data_ptr(), w.stride(0), w.shape[1], p)
+        return xs, scales
+
+    def _front_int8(self, x, p0: int):
+        """q (B,H,L,Dh) before RoPE, k (B,Hkv,L,Dh) roped, v, the gate (B,L)
+        float32 (None without one), lambda (B,H,L) and the RoPE tables of
+        positions p0 .., of x (B,L,D), a tensor or Int8Rows."""
+        B, L = x.shape[:2]
+        H, Hkv, Dh, dt, dev = self.num_heads, self.num_kv_heads, self.head_dim, x.dtype, x.device
+        cos, sin = self._rope_tables(p0, L, dev, dt)
         Fq, Fk = H * Dh, Hkv * Dh
         q = torch.empty((B, L, H, Dh), dtype=dt, device=dev)
         k = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
         v = torch.empty((B, L, Hkv, Dh), dtype=dt, device=dev)
         lam = torch.empty((B, L, H), dtype=dt, device=dev)
         g = torch.empty((B, L), dtype=torch.float32, device=dev) if self._has_gate() else None
-        codes, sm, scales = _flat(r) if isinstance(r, Int8Rows) else (*_rows_of(r), None)
-        d = self._proj_desc(r, B * L, L, cos, sin)
-        params = None
-        if tables is not None:
-            params, d.rope_cos, d.rope_sin = tables
-        d.w, d.bias = w.data_ptr(), bias.data_ptr()
-        d.x, d.x_sm = codes.data_ptr(), sm
+        d = self._proj_desc(x, B * L, L, cos, sin)
         d.q, d.q_sm, d.k, d.k_sm, d.v, d.v_sm = q.data_ptr(), Fq, k.data_ptr(), Fk, v.data_ptr(), Fk
         d.lam, d.lam_sm, d.g = lam.data_ptr(), H, _hip.ptr(g)
-        _call(_hip.lib().coda_project_int8, codes, d, _hip.ptr(scales), sw.data_ptr(), w.stride(0), w.shape[1],
-              params)
+        self._launch_int8(x, d, self._int8_weights())
         return (q.permute(0, 2, 1, 3), k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3), g, lam.permute(0, 2, 1), cos, sin)
 
-    def _out_proj(self, heads: torch.Tensor) -> torch.Tensor:
-        """o_proj of heads (B, L, H*Dh): the module, or in 8 bits."""
+    def _out_proj(self, heads: torch.Tensor, weights: Optional[tuple] = None) -> torch.Tensor:
+        """o_proj of heads (B, L, H*Dh): the module, or in 8 bits (weights:
+        _int8_weights() of this call)."""
         if not self.int8_projections:
             return self.o_proj(heads)
-        w, sw, bias = self._int8_weights()[3:]
+        w, sw, bias = (weights or self._int8_weights())[3:]
         return linear_int8(heads, _made(w, sw, heads.shape[-1], heads.dtype), bias)

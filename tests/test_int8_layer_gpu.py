@@ -272,7 +272,8 @@ def test_refused():
 # ---------------------------------------------------------------- unbounded layer
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,L,past,causal", [(1, 1, 0, True), (2, 65, 0, True), (1, 300, 0, False), (2, 3, 50, False),
-                                             (3, 1, 120, False), (2, 20, 40, False)])
+                                             (3, 1, 120, False), (2, 20, 40, False), (200, 1, 30, False),
+                                             (70, 2, 30, False)])
 @torch.no_grad()
 def test_unbounded(B, L, past, causal, dtype):
     m = _unbounded(dtype)
@@ -285,7 +286,7 @@ def test_unbounded(B, L, past, causal, dtype):
     assert torch.equal(k, ks) and torch.equal(v, vs)
     heads = m.attention_core(q, ks, vs, lam, cos, sin, causal=2 if causal else 0)
     want = _out(m, heads)
-    if dtype == torch.bfloat16 and past and L * 4 <= 8:
+    if dtype == torch.bfloat16 and past and L * 4 <= 8 and B * L <= 128:
         # another attention kernel: heads within the layer's bound, and codes
         # of heads that differ by it
         assert (y.float() - want.float()).abs().max() <= 4e-2 * want.float().abs().max()
