@@ -479,6 +479,9 @@ template <int N>
 __device__ __forceinline__ void tile_landed(i32x4 (&a)[N]) {
   if constexpr (N == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]));
   if constexpr (N == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+  if constexpr (N == 6)
+    asm volatile("s_waitcnt lgkmcnt(0)"
+                 : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]));
   if constexpr (N == 8)
     asm volatile("s_waitcnt lgkmcnt(0)"
                  : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7]));
@@ -501,38 +504,38 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
   return v;
 }
 
-// 4 waves (2 x 2) make 64 S features x 64 S tokens, a wave 32 S x 32 S in
-// S x S accumulators of 32 x 32.  K passes through LDS in steps of 64 bytes,
+// 4 waves (2 x 2) make 64 SF features x 64 SM tokens, a wave 32 SF x 32 SM in
+// SF x SM accumulators of 32 x 32.  K passes through LDS in steps of 64 bytes,
 // four stages: while the products of step k run, step k + 1 lies in LDS
 // (its first operands are read ahead, so that no product waits for LDS after
 // a barrier), step k + 2 is on its way and step k + 3 is asked for: one
 // barrier a step.  A stage holds a row's four 16-byte pieces in the order
 // slot = piece ^ (row / 4) % 4, by which the 16 lanes that LDS serves at once
 // (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
-// A workgroup of the largest tile (S = 4: one a CU) goes from tile to tile;
+// A workgroup of the larger tiles (SF = 4: one a CU) goes from tile to tile;
 // the stages run on over the border, so that the next tile's first steps are
 // in LDS when this one's values have been written, and the writes are on
 // their way while its products run.
-template <int S, typename T>
+template <int SF, int SM, typename T>
 struct TileLds {
-  static constexpr int kRows = 128 * S;       // features, then tokens
-  static constexpr int kStage = kRows * 64;   // bytes
-  static constexpr bool kWalk = S == 4;
+  static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
+  static constexpr int kStage = kRows * 64;     // bytes
+  static constexpr bool kWalk = SF == 4;
   // a wave's values on their way out: 32 tokens x kFeats features
-  static constexpr int kFeats = kWalk ? 128 / (int)sizeof(T) : 32 * S;
+  static constexpr int kFeats = kWalk ? 128 / (int)sizeof(T) : 32 * SF;
   static constexpr int kRow = kFeats * sizeof(T) + 16;
-  static constexpr int kScales = 3 * 64 * S * sizeof(float);  // features' scales, biases, tokens' scales
+  static constexpr int kScales = 64 * (2 * SF + SM) * sizeof(float);  // features' scales, biases, tokens' scales
   static constexpr int kOut = kWalk ? 4 * kStage : 0;         // (smaller tiles: over the stages)
   static constexpr size_t kEnd = kOut + kScales + 4 * 32 * kRow;
   static constexpr size_t kBytes = kEnd > 4 * kStage ? kEnd : 4 * kStage;
 };
-template <int S, typename Sink>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 : 2))) void int8_tile(
+template <int SF, int SM, typename Sink>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1 : 2))) void int8_tile(
     const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
   typedef typename Sink::Out T;
-  typedef TileLds<S, T> L;
+  typedef TileLds<SF, SM, T> L;
   extern __shared__ __attribute__((aligned(128))) char smem[];
-  constexpr int BF = 64 * S, BM = 64 * S, NL = L::kRows / 64;  // loads a thread and step
+  constexpr int BF = 64 * SF, BM = 64 * SM, NL = SF + SM;  // NL loads a thread and step
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
   // in groups of 4 token tiles, so that what it has at a time shares rows in
@@ -548,7 +551,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
     return At{in / gm * BF, (4 * group + in % gm) * BM};
   };
   // this lane's pieces, as offsets from a tile's first rows: a load is 16 rows
-  // of four pieces, the first half of them features
+  // of four pieces, the first SF of them features
   uint32_t src[NL];
   const int8_t *wsrc, *xsrc;
   auto aim = [&](const At& a) {
@@ -556,8 +559,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
     asm volatile("" : "+v"(l));  // (nothing of this is worth a register between tiles)
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int r = (4 * (i % S) + wv) * 16 + (l >> 2), piece = (l & 3) ^ ((r >> 2) & 3);
-      src[i] = 16 * piece + (i < S ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
+      const int r = (4 * (i < SF ? i : i - SF) + wv) * 16 + (l >> 2), piece = (l & 3) ^ ((r >> 2) & 3);
+      src[i] = 16 * piece + (i < SF ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
                                    : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
     }
     wsrc = W.p + a.f * W.sm;
@@ -568,7 +571,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
   int tile = t0 + (int)(blockIdx.x >> 3), lt = tile, lk = 0, ls = 0;
   auto load1 = [&](auto c) {
     constexpr int i = decltype(c)::value;
-    tile_load16((i < S ? wsrc : xsrc) + src[i], smem + (ls & 3) * L::kStage + wv * 1024 + i * 4096);
+    tile_load16((i < SF ? wsrc : xsrc) + src[i], smem + (ls & 3) * L::kStage + wv * 1024 + i * 4096);
   };
   auto loaded = [&]() {
     ++ls;
@@ -580,32 +583,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
       if (lt < end) aim(place(lt));
     }
   };
-  i32x16 acc[S][S];
+  i32x16 acc[SF][SM];
   // operands of half h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
   const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 2) & 3)) << 4);
-  i32x4 op[2][2 * S];
-  auto read = [&](auto c, i32x4 (&o)[2 * S], uint32_t a) {  // operand c: S of features, S of tokens
+  i32x4 op[2][NL];
+  auto read = [&](auto c, i32x4 (&o)[NL], uint32_t a) {  // operand c: SF of features, SM of tokens
     constexpr int i = decltype(c)::value;
-    o[i] = i < S ? tile_read<i * 2048>(a + wf * (S * 2048)) : tile_read<BF * 64 + (i - S) * 2048>(a + wm * (S * 2048));
+    if constexpr (i < SF) o[i] = tile_read<i * 2048>(a + wf * (SF * 2048));
+    else o[i] = tile_read<BF * 64 + (i - SF) * 2048>(a + wm * (SM * 2048));
   };
   // Products of half h of a step, and beside them the reads of the next half
   // (early, so that they land before its first product) and half of a later
   // step's loads (late and apart: asked for all at once before the products,
   // they hold the wave up for as long as half of the products take).
-  auto half = [&](auto hc, auto more, i32x4 (&now)[2 * S], i32x4 (&next)[2 * S], uint32_t a) {
+  auto half = [&](auto hc, auto more, i32x4 (&now)[NL], i32x4 (&next)[NL], uint32_t a) {
     constexpr int h = decltype(hc)::value;
-    each<S * S>([&](auto c) {
-      constexpr int q = decltype(c)::value, i = q / S, j = q % S;
-      constexpr int reads = S == 4 ? 1 : 2;                   // a product
-      constexpr int first = S * S / 2, gap = S == 4 ? 2 : 1;  // loads beside products first, first + gap ..
+    each<SF * SM>([&](auto c) {
+      constexpr int n = SF * SM, q = decltype(c)::value, i = q / SM, j = q % SM;
+      constexpr int reads = n >= 2 * NL ? 1 : 2;                        // a product
+      constexpr int first = n / 2, gap = n >= 2 * NL ? n / NL : 1;      // loads beside products first, first + gap ..
       each<reads>([&](auto d) {
         constexpr int o = q * reads + decltype(d)::value;
-        if constexpr (o < 2 * S) read(std::integral_constant<int, o>{}, next, a);
+        if constexpr (o < NL) read(std::integral_constant<int, o>{}, next, a);
       });
-      if constexpr (decltype(more)::value && q >= first && (q - first) % gap == 0)
+      if constexpr (decltype(more)::value && q >= first && (q - first) % gap == 0 && (q - first) / gap < NL / 2)
         load1(std::integral_constant<int, h * (NL / 2) + (q - first) / gap>{});
-      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[S + j], acc[i][j], 0, 0, 0);
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[SF + j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
     tile_landed(next);
@@ -635,7 +639,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
   if (ls == 3) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
   else __builtin_amdgcn_s_waitcnt(0x0f70);
   __builtin_amdgcn_s_barrier();
-  each<2 * S>([&](auto c) { read(c, op[0], at); });
+  each<NL>([&](auto c) { read(c, op[0], at); });
   tile_landed(op[0]);
   for (;;) {
     const At a = place(tile);
@@ -645,12 +649,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
       const int f = min(a.f + own, W.rows - 1);
       scale[0] = W.scales[f];
       scale[1] = sink.bias1(f);
-      scale[2] = X.scales[min(a.m + own, X.rows - 1)];
     }
+    if (own < BM) scale[2] = X.scales[min(a.m + own, X.rows - 1)];
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+    for (int i = 0; i < SF; ++i)
 #pragma unroll
-      for (int j = 0; j < S; ++j)
+      for (int j = 0; j < SM; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
     int k = 0;
@@ -669,20 +673,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
     if (own < BF) {
       fs[own] = scale[0];
       fs[BF + own] = scale[1];
-      fs[2 * BF + own] = scale[2];
     }
+    if (own < BM) fs[2 * BF + own] = scale[2];
     // every load so far has landed: the writes below do not hold up the
     // next steps' waits
     __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
     constexpr int N = Sink::kRun, PR = L::kFeats / N, NF = L::kFeats / 32;  // runs of a row, blocks of 32 features
     char* mine = smem + L::kOut + L::kScales + wv * 32 * L::kRow;
-    const int fw = 32 * S * wf, mw = 32 * S * wm, fq = le % PR * N;
+    const int fw = 32 * SF * wf, mw = 32 * SM * wm, fq = le % PR * N;
     const float* fl = fs + fw + 4 * (le >> 5);
-    each<S>([&](auto jc) {
+    each<SM>([&](auto jc) {
       constexpr int j = decltype(jc)::value;
       const float sx = fs[2 * BF + mw + 32 * j + (le & 31)];
-      each<S / NF>([&](auto pc) {
+      each<SF / NF>([&](auto pc) {
         constexpr int part = decltype(pc)::value;
         each<4 * NF>([&](auto gc) {
           constexpr int q = decltype(gc)::value, i = part * NF + q / 4, r = q % 4, f = 32 * i + 8 * r;
@@ -714,16 +718,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(S == 4 ? 1 
   }
 }
 
-template <int S, typename Sink>
+template <int SF, int SM, typename Sink>
 static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  typedef TileLds<S, typename Sink::Out> L;
-  const int64_t ntf = ((int64_t)W.rows + 64 * S - 1) / (64 * S), ntm = ((int64_t)X.rows + 64 * S - 1) / (64 * S);
+  typedef TileLds<SF, SM, typename Sink::Out> L;
+  const int64_t ntf = ((int64_t)W.rows + 64 * SF - 1) / (64 * SF), ntm = ((int64_t)X.rows + 64 * SM - 1) / (64 * SM);
   const int64_t n = ntf * ntm;
   if (n > INT_MAX / 8) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
-  const int rc = lds_limit<int8_tile<S, Sink>>(L::kBytes, who);
+  const int rc = lds_limit<int8_tile<SF, SM, Sink>>(L::kBytes, who);
   if (rc) return rc;
   const int64_t grid = L::kWalk && n > device_cus() ? device_cus() : n;
-  hipLaunchKernelGGL((int8_tile<S, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
+  hipLaunchKernelGGL((int8_tile<SF, SM, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
                      sink);
   return check_launch("int8_tile");
 }
@@ -866,10 +870,11 @@ template <typename Sink>
 static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
   // the largest tile that gives every CU one
   const int cus = device_cus();
-  auto tiles = [&](int b) { return ((int64_t)W.rows + b - 1) / b * (((int64_t)X.rows + b - 1) / b); };
-  if (tiles(256) >= cus) return launch_tile<4>(X, W, K, sink, st, who);
-  if (tiles(128) >= cus) return launch_tile<2>(X, W, K, sink, st, who);
-  return launch_tile<1>(X, W, K, sink, st, who);
+  auto tiles = [&](int f, int m) { return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m); };
+  if (tiles(256, 256) >= cus) return launch_tile<4, 4>(X, W, K, sink, st, who);
+  if (tiles(256, 128) >= cus) return launch_tile<4, 2>(X, W, K, sink, st, who);
+  if (tiles(128, 128) >= cus) return launch_tile<2, 2>(X, W, K, sink, st, who);
+  return launch_tile<1, 1>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {
