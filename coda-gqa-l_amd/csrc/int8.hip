@@ -505,37 +505,40 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 }
 
 // 4 waves (2 x 2) make 64 SF features x 64 SM tokens, a wave 32 SF x 32 SM in
-// SF x SM accumulators of 32 x 32.  K passes through LDS in steps of 64 bytes,
-// four stages: while the products of step k run, step k + 1 lies in LDS
-// (its first operands are read ahead, so that no product waits for LDS after
-// a barrier), step k + 2 is on its way and step k + 3 is asked for: one
-// barrier a step.  A stage holds a row's four 16-byte pieces in the order
-// slot = piece ^ (row / 4) % 4, by which the 16 lanes that LDS serves at once
-// (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
+// SF x SM accumulators of 32 x 32.  K passes through LDS in steps of 128 bytes
+// (whole lines: rows of 64 bytes come out of L2 at 70 GB/s a CU, of 128 at
+// 120), ST stages.  A step is four quarters of 32 bytes of K.  Beside a
+// quarter's products the next one's operands are read, so that none waits for
+// LDS.  The one barrier of a step is before its last quarter: by then every
+// wave has read all of the step, whose stage is loaded anew (step + ST) beside
+// that quarter and the next two, and the next step, whose first operands are
+// read now, has landed.  A stage holds a row's eight 16-byte pieces in the
+// order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
+// once (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
 // A workgroup of the larger tiles (SF = 4: one a CU) goes from tile to tile;
 // the stages run on over the border, so that the next tile's first steps are
 // in LDS when this one's values have been written, and the writes are on
 // their way while its products run.
-template <int SF, int SM, typename T>
+template <int SF, int SM, int ST, typename T>
 struct TileLds {
   static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
-  static constexpr int kStage = kRows * 64;     // bytes
+  static constexpr int kStage = kRows * 128;    // bytes
   static constexpr bool kWalk = SF == 4;
   // a wave's values on their way out: 32 tokens x kFeats features
   static constexpr int kFeats = kWalk ? 128 / (int)sizeof(T) : 32 * SF;
   static constexpr int kRow = kFeats * sizeof(T) + 16;
   static constexpr int kScales = 64 * (2 * SF + SM) * sizeof(float);  // features' scales, biases, tokens' scales
-  static constexpr int kOut = kWalk ? 4 * kStage : 0;         // (smaller tiles: over the stages)
+  static constexpr int kOut = kWalk ? ST * kStage : 0;         // (smaller tiles: over the stages)
   static constexpr size_t kEnd = kOut + kScales + 4 * 32 * kRow;
-  static constexpr size_t kBytes = kEnd > 4 * kStage ? kEnd : 4 * kStage;
+  static constexpr size_t kBytes = kEnd > ST * kStage ? kEnd : ST * kStage;
 };
-template <int SF, int SM, typename Sink>
+template <int SF, int SM, int ST, typename Sink>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1 : 2))) void int8_tile(
     const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
   typedef typename Sink::Out T;
-  typedef TileLds<SF, SM, T> L;
+  typedef TileLds<SF, SM, ST, T> L;
   extern __shared__ __attribute__((aligned(128))) char smem[];
-  constexpr int BF = 64 * SF, BM = 64 * SM, NL = SF + SM;  // NL loads a thread and step
+  constexpr int BF = 64 * SF, BM = 64 * SM, NO = SF + SM, NL = 2 * NO;  // NO operands a quarter, NL loads a thread and step
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
   // in groups of 4 token tiles, so that what it has at a time shares rows in
@@ -550,8 +553,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
     const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
     return At{in / gm * BF, (4 * group + in % gm) * BM};
   };
-  // this lane's pieces, as offsets from a tile's first rows: a load is 16 rows
-  // of four pieces, the first SF of them features
+  // this lane's pieces, as offsets from a tile's first rows: a load is 8 rows
+  // of eight pieces, the first 2 SF of them features
   uint32_t src[NL];
   const int8_t *wsrc, *xsrc;
   auto aim = [&](const At& a) {
@@ -559,24 +562,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
     asm volatile("" : "+v"(l));  // (nothing of this is worth a register between tiles)
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int r = (4 * (i < SF ? i : i - SF) + wv) * 16 + (l >> 2), piece = (l & 3) ^ ((r >> 2) & 3);
-      src[i] = 16 * piece + (i < SF ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
-                                   : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
+      const int r = (4 * (i < 2 * SF ? i : i - 2 * SF) + wv) * 8 + (l >> 3), piece = (l & 7) ^ ((r >> 1) & 7);
+      src[i] = 16 * piece + (i < 2 * SF ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
+                                        : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
     }
     wsrc = W.p + a.f * W.sm;
     xsrc = X.p + a.m * X.sm;
   };
-  // the loads: tile lt's step lk into stage ls; on to the next tile at its end
-  const int steps = K / 64;
-  int tile = t0 + (int)(blockIdx.x >> 3), lt = tile, lk = 0, ls = 0;
+  // the loads: tile lt's step lk, the ls-th of all, to stage lat; on to the next
+  // tile at its end
+  const int steps = K / 128;
+  int tile = t0 + (int)(blockIdx.x >> 3), lt = tile, lk = 0, ls = 0, lat = 0;
   auto load1 = [&](auto c) {
     constexpr int i = decltype(c)::value;
-    tile_load16((i < SF ? wsrc : xsrc) + src[i], smem + (ls & 3) * L::kStage + wv * 1024 + i * 4096);
+    tile_load16((i < 2 * SF ? wsrc : xsrc) + src[i], smem + lat + wv * 1024 + i * 4096);
   };
+  auto next_stage = [](int at) { return at + L::kStage == ST * L::kStage ? 0 : at + L::kStage; };
   auto loaded = [&]() {
     ++ls;
-    wsrc += 64;
-    xsrc += 64;
+    lat = next_stage(lat);
+    wsrc += 128;
+    xsrc += 128;
     if (++lk == steps) {
       lk = 0;
       lt = L::kWalk ? lt + turn : end;
@@ -584,62 +590,80 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
     }
   };
   i32x16 acc[SF][SM];
-  // operands of half h of a step: pieces 2 h + lane / 32
+  // operands of quarter h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
-  const uint32_t at = tile_lds(smem) + r32 * 64 + (((lane >> 5) ^ ((r32 >> 2) & 3)) << 4);
-  i32x4 op[2][NL];
-  auto read = [&](auto c, i32x4 (&o)[NL], uint32_t a) {  // operand c: SF of features, SM of tokens
+  const uint32_t at = tile_lds(smem) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
+  i32x4 op[2][NO];
+  auto read = [&](auto c, i32x4 (&o)[NO], uint32_t a) {  // operand c: SF of features, SM of tokens
     constexpr int i = decltype(c)::value;
-    if constexpr (i < SF) o[i] = tile_read<i * 2048>(a + wf * (SF * 2048));
-    else o[i] = tile_read<BF * 64 + (i - SF) * 2048>(a + wm * (SM * 2048));
+    if constexpr (i < SF) o[i] = tile_read<i * 4096>(a + wf * (SF * 4096));
+    else o[i] = tile_read<BF * 128 + (i - SF) * 4096>(a + wm * (SM * 4096));
   };
-  // Products of half h of a step, and beside them the reads of the next half
-  // (early, so that they land before its first product) and half of a later
-  // step's loads (late and apart: asked for all at once before the products,
-  // they hold the wave up for as long as half of the products take).
-  auto half = [&](auto hc, auto more, i32x4 (&now)[NL], i32x4 (&next)[NL], uint32_t a) {
-    constexpr int h = decltype(hc)::value;
-    each<SF * SM>([&](auto c) {
-      constexpr int n = SF * SM, q = decltype(c)::value, i = q / SM, j = q % SM;
-      constexpr int reads = n >= 2 * NL ? 1 : 2;                        // a product
-      constexpr int first = n / 2, gap = n >= 2 * NL ? n / NL : 1;      // loads beside products first, first + gap ..
+  // The products of a quarter; beside the first of them the reads of the next
+  // one's operands, at address a; beside the last loads from .. to of the step
+  // that is asked for (asked for all at once, they hold the wave up).
+  auto quarter = [&](auto from, auto to, bool some, i32x4 (&now)[NO], i32x4 (&next)[NO], uint32_t a) {
+    constexpr int n = SF * SM, lo = decltype(from)::value, hi = decltype(to)::value;
+    constexpr int reads = n >= 2 * NO ? 1 : 2, first = n / 2, loads = (hi - lo + n - first - 1) / (n - first);
+    each<n>([&](auto c) {
+      constexpr int q = decltype(c)::value, i = q / SM, j = q % SM;
       each<reads>([&](auto d) {
         constexpr int o = q * reads + decltype(d)::value;
-        if constexpr (o < NL) read(std::integral_constant<int, o>{}, next, a);
+        if constexpr (o < NO) read(std::integral_constant<int, o>{}, next, a);
       });
-      if constexpr (decltype(more)::value && q >= first && (q - first) % gap == 0 && (q - first) / gap < NL / 2)
-        load1(std::integral_constant<int, h * (NL / 2) + (q - first) / gap>{});
+      if constexpr (q >= first && lo + (q - first) * loads < hi)
+        if (some)
+          each<loads>([&](auto d) {
+            constexpr int o = lo + (q - first) * loads + decltype(d)::value;
+            if constexpr (o < hi) load1(std::integral_constant<int, o>{});
+          });
       acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[i], now[SF + j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
     tile_landed(next);
   };
-  // At the start of step g: g + 1 has landed for every wave, all are done with
-  // g - 1.  more: the loads are three steps ahead still; wait: for g + 2, the
-  // last but one that was asked for (or, without more, the last).
-  int g = 0;
-  auto step = [&](auto more, auto wait) {
-    const uint32_t here = at + (g & 3) * L::kStage, then = at + ((g + 1) & 3) * L::kStage;
-    half(std::integral_constant<int, 0>{}, more, op[0], op[1], here ^ 32);
-    half(std::integral_constant<int, 1>{}, more, op[1], op[0], then);
-    if constexpr (decltype(more)::value) loaded();
-    if constexpr (decltype(wait)::value && decltype(more)::value) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
-    else if constexpr (decltype(wait)::value) __builtin_amdgcn_s_waitcnt(0x0f70);
+  // steps up to n have landed: those asked for behind it may be on their way
+  auto landed = [&](int n) {
+    const int behind = ls - 1 - n;
+    if (behind <= 0) __builtin_amdgcn_s_waitcnt(0x0f70);
+    each<ST - 2>([&](auto c) {
+      constexpr int v = (decltype(c)::value + 1) * NL;
+      static_assert(v < 64, "vmcnt is 6 bits");
+      if (behind == decltype(c)::value + 1) __builtin_amdgcn_s_waitcnt((v & 15) | (v >> 4) << 14 | 0x0f70);
+    });
+  };
+  // Step g, in stage rat.  asked: a third of a step was asked for at the end of
+  // the last one.
+  int g = 0, rat = 0;
+  bool asked = false;
+  auto step = [&]() {
+    constexpr int third = (NL + 2) / 3;
+    constexpr std::integral_constant<int, 0> none{};
+    constexpr std::integral_constant<int, third> one{};
+    constexpr std::integral_constant<int, 2 * third> two{};
+    constexpr std::integral_constant<int, NL> all{};
+    const uint32_t here = at + rat;
+    rat = next_stage(rat);
+    quarter(one, two, asked, op[0], op[1], here ^ 32);
+    quarter(two, all, asked, op[1], op[0], here ^ 64);
+    if (asked) loaded();
+    quarter(none, none, false, op[0], op[1], here ^ 96);
+    landed(g + 1);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    asked = lt < end;
+    quarter(none, one, asked, op[1], op[0], at + rat);
     ++g;
   };
   aim(place(tile));
-  for (int s = 0; s < 3 && lt < end; ++s) {
+  for (int s = 0; s < ST && lt < end; ++s) {
     each<NL>([&](auto c) { load1(c); });
     loaded();
   }
   __builtin_amdgcn_sched_barrier(0);
-  // steps 0 and 1 have landed (K is a multiple of 128: there are two)
-  if (ls == 3) __builtin_amdgcn_s_waitcnt((NL & 15) | 0x0f70);
-  else __builtin_amdgcn_s_waitcnt(0x0f70);
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   __builtin_amdgcn_s_barrier();
-  each<NL>([&](auto c) { read(c, op[0], at); });
+  each<NO>([&](auto c) { read(c, op[0], at); });
   tile_landed(op[0]);
   for (;;) {
     const At a = place(tile);
@@ -657,26 +681,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
       for (int j = 0; j < SM; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    int k = 0;
-    // (a later tile: its second step has landed before the values were written)
-    if (g > 0 && lt < end) {
-      step(std::true_type{}, std::false_type{});
-      ++k;
-    }
-    for (; k < steps && lt < end; ++k) step(std::true_type{}, std::true_type{});
-    for (; k < steps; ++k) step(std::false_type{}, std::true_type{});
+    for (int k = 0; k < steps; ++k) step();
     // Values pass through LDS (a wave's own part) from four features of 32
     // tokens a lane to runs of a token's features
     int le = lane;
     asm volatile("" : "+v"(le));  // (nor are these addresses)
+    if (!L::kWalk) __builtin_amdgcn_s_barrier();  // every wave has read its last operands
     float* fs = reinterpret_cast<float*>(smem + L::kOut);
     if (own < BF) {
       fs[own] = scale[0];
       fs[BF + own] = scale[1];
     }
     if (own < BM) fs[2 * BF + own] = scale[2];
-    // every load so far has landed: the writes below do not hold up the
-    // next steps' waits
+    // (the loads too: the writes below do not stand before them)
     __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
     constexpr int N = Sink::kRun, PR = L::kFeats / N, NF = L::kFeats / 32;  // runs of a row, blocks of 32 features
@@ -718,16 +735,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   }
 }
 
-template <int SF, int SM, typename Sink>
+template <int SF, int SM, int ST, typename Sink>
 static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  typedef TileLds<SF, SM, typename Sink::Out> L;
+  typedef TileLds<SF, SM, ST, typename Sink::Out> L;
   const int64_t ntf = ((int64_t)W.rows + 64 * SF - 1) / (64 * SF), ntm = ((int64_t)X.rows + 64 * SM - 1) / (64 * SM);
   const int64_t n = ntf * ntm;
   if (n > INT_MAX / 8) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
-  const int rc = lds_limit<int8_tile<SF, SM, Sink>>(L::kBytes, who);
+  const int rc = lds_limit<int8_tile<SF, SM, ST, Sink>>(L::kBytes, who);
   if (rc) return rc;
   const int64_t grid = L::kWalk && n > device_cus() ? device_cus() : n;
-  hipLaunchKernelGGL((int8_tile<SF, SM, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
+  hipLaunchKernelGGL((int8_tile<SF, SM, ST, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
                      sink);
   return check_launch("int8_tile");
 }
@@ -871,10 +888,10 @@ static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   // the largest tile that gives every CU one
   const int cus = device_cus();
   auto tiles = [&](int f, int m) { return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m); };
-  if (tiles(256, 256) >= cus) return launch_tile<4, 4>(X, W, K, sink, st, who);
-  if (tiles(256, 128) >= cus) return launch_tile<4, 2>(X, W, K, sink, st, who);
-  if (tiles(128, 128) >= cus) return launch_tile<2, 2>(X, W, K, sink, st, who);
-  return launch_tile<1, 1>(X, W, K, sink, st, who);
+  if (tiles(256, 256) >= cus) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
+  if (tiles(256, 128) >= cus) return launch_tile<4, 2, 2>(X, W, K, sink, st, who);
+  if (tiles(128, 128) >= cus) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
+  return launch_tile<1, 1, 4>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {
