@@ -145,7 +145,11 @@ def _rows_of(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
 def _new_rows(x: torch.Tensor, D: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
     """Uninitialised codes and scales of x's rows, and the codes of a row."""
     lead, P, dev = x.shape[:-1], _padded(D), x.device
-    return torch.empty((*lead, P), dtype=torch.int8, device=dev), torch.empty(lead, dtype=torch.float32, device=dev), P
+    if P == D and x.is_contiguous():
+        codes = torch.empty_like(x, dtype=torch.int8)
+    else:
+        codes = torch.empty((*lead, P), dtype=torch.int8, device=dev)
+    return codes, torch.empty(lead, dtype=torch.float32, device=dev), P
 
 
 def _check_input(x: torch.Tensor, who: str) -> int:
@@ -184,9 +188,10 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         raise RuntimeError(f"rms_norm_int8: weight {tuple(weight.shape)}, expected ({D},)")
     if residual is not None and residual.shape != x.shape:
         raise RuntimeError(f"rms_norm_int8: residual {tuple(residual.shape)} is not x's shape {tuple(x.shape)}")
-    for name, t in (("weight", weight), ("residual", residual)):
-        if t is not None and (t.dtype is not dt or t.device != x.device):
-            raise RuntimeError(f"rms_norm_int8: {name} is {t.dtype} on {t.device}, x {dt} on {x.device}")
+    if weight.dtype is not dt or weight.device != x.device:
+        raise RuntimeError(f"rms_norm_int8: weight is {weight.dtype} on {weight.device}, x {dt} on {x.device}")
+    if residual is not None and (residual.dtype is not dt or residual.device != x.device):
+        raise RuntimeError(f"rms_norm_int8: residual is {residual.dtype} on {residual.device}, x {dt} on {x.device}")
     if not eps >= 0:
         raise RuntimeError(f"rms_norm_int8: eps={eps} is negative")
     x2, sm = _rows_of(x)
@@ -198,7 +203,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
               codes.data_ptr(), P, scales.data_ptr())
         return _made(codes, scales, D, dt)
     r2, rm = _rows_of(residual)
-    out = torch.empty(x.shape, dtype=dt, device=x.device)
+    out = torch.empty_like(x2) if x2 is x else torch.empty(x.shape, dtype=dt, device=x.device)
     _call(fn, x, code, x2.data_ptr(), sm, r2.data_ptr(), rm, w.data_ptr(), scales.numel(), D, float(eps),
           out.data_ptr(), D, codes.data_ptr(), P, scales.data_ptr())
     return _made(codes, scales, D, dt), out

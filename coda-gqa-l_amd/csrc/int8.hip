@@ -515,7 +515,7 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // read now, has landed.  A stage holds a row's eight 16-byte pieces in the
 // order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
 // once (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
-// A workgroup of the larger tiles (SF = 4: one a CU) goes from tile to tile;
+// A workgroup of the largest tiles goes from tile to tile;
 // the stages run on over the border, so that the next tile's first steps are
 // in LDS when this one's values have been written, and the writes are on
 // their way while its products run.
@@ -523,7 +523,7 @@ template <int SF, int SM, int ST, typename T>
 struct TileLds {
   static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
   static constexpr int kStage = kRows * 128;    // bytes
-  static constexpr bool kWalk = SF == 4;
+  static constexpr bool kWalk = SF * SM == 16;
   // a wave's values on their way out: 32 tokens x kFeats features
   static constexpr int kFeats = kWalk ? 128 / (int)sizeof(T) : 32 * SF;
   static constexpr int kRow = kFeats * sizeof(T) + 16;
@@ -712,7 +712,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
           i32x4 v;
           each<4>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
-            v[e] = L::kWalk ? acc_read(acc[i][j][4 * r + e]) : acc[i][j][4 * r + e];
+            v[e] = SF == 4 ? acc_read(acc[i][j][4 * r + e]) : acc[i][j][4 * r + e];
           });
           *reinterpret_cast<Feats<T, 4>*>(mine + (le & 31) * L::kRow + (32 * (q / 4) + 8 * r + 4 * (le >> 5)) * sizeof(T)) =
               int8_value<T>(v, sx, sw, bias);
@@ -877,20 +877,37 @@ static int launch_of(const void* x, int64_t x_sm, int M, int D, const Int8Mat& W
   }
 }
 
-static constexpr int kFewRows = 128;
+static constexpr int kFewRows = 128;  // of the row kernels
 template <typename Sink>
 static int launch_few(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
   return launch_rows<int8_t>(MatRows<int8_t>{W.p, W.sm}, W.rows, K, X.p, X.sm, X.rows,
                              RowsSink<Sink>{sink, X.scales, W.scales, W.rows}, st, who);
 }
+static int64_t tiles_of(const Int8Mat& X, const Int8Mat& W, int f, int m) {
+  return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m);
+}
+// Whether the row kernels or the smallest tiles: up to 64 rows the former, up
+// to 128 where the tiles do not go round in one (us, rows and tiles: 17 x 4096
+// x 6177 11.5 and 14.2, 64 x 4096 x 4096 10.0 and 13.6, 64 x 4096 x 6177 14.6
+// both, 128 x 4096 x 6177 19.2 and 14.9, 128 x 8192 x 8192 32.0 and 27.1, 128
+// x 8192 x 10305, 322 tiles, 38.1 and 40.9).
+static bool few_rows(const Int8Mat& X, const Int8Mat& W) {
+  return X.rows <= 64 || (X.rows <= kFewRows && tiles_of(X, W, 64, 64) > device_cus());
+}
+// The tile by the time that its rounds take, us a round of one tile (64 x 64:
+// two) a CU at K = 4096.  Measured, 256 x 256 | 256 x 128 | 128 x 128 | 64 x
+// 64: 1999 x 4096 x 4096 55 41 50 75, 1999 x 4096 x 6177 58 68 81 107, 1000 x
+// 4096 x 4096 52 31 24 38, 300 x 4096 x 6177 - - 20 21, 500 x 2048 x 3105 - -
+// 12.5 11.3, 4096 x 4096 x 6177 112 130 - -, 2000 x 1024 x 1024 - - 9.3 8.1.
 template <typename Sink>
 static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  // the largest tile that gives every CU one
-  const int cus = device_cus();
-  auto tiles = [&](int f, int m) { return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m); };
-  if (tiles(256, 256) >= cus) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
-  if (tiles(256, 128) >= cus) return launch_tile<4, 2, 2>(X, W, K, sink, st, who);
-  if (tiles(128, 128) >= cus) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
+  const int64_t cus = device_cus(), n1 = tiles_of(X, W, 64, 64);
+  const auto rounds = [&](int f, int m) { return (tiles_of(X, W, f, m) + cus - 1) / cus; };
+  const int64_t t44 = 56 * rounds(256, 256), t42 = 39 * rounds(256, 128), t22 = 23 * rounds(128, 128);
+  const int64_t t11 = n1 <= cus ? 15 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
+  if (t44 <= t42 && t44 <= t22 && t44 <= t11) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
+  if (t42 <= t22 && t42 <= t11) return launch_tile<4, 2, 3>(X, W, K, sink, st, who);
+  if (t22 <= t11) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
   return launch_tile<1, 1, 4>(X, W, K, sink, st, who);
 }
 
@@ -987,8 +1004,8 @@ extern "C" int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const fl
     typedef decltype(t) T;
     const LinearSink<T> sink{(T*)out, (const T*)bias, o_sm, n_feat};
     return !x_scales       ? launch_of<T>(x, x_sm, M, D, W, K, sink, st, who)
-           : M <= kFewRows ? launch_few(X, W, K, sink, st, who)
-                           : launch_many(X, W, K, sink, st, who);
+           : few_rows(X, W) ? launch_few(X, W, K, sink, st, who)
+                            : launch_many(X, W, K, sink, st, who);
   };
   return dtype == CODA_F32 ? run(float{}) : dtype == CODA_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
@@ -1026,10 +1043,9 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
   const FastDiv len(d->L);
   const auto run = [&](auto t) {
     typedef decltype(t) T;
-    if (d->M <= kFewRows) {
-      const FrontSink<T, true, 4> sink{*d, tab, len, n_feat};
-      return x_scales ? launch_few(X, W, K, sink, st, who) : launch_of<T>(d->x, d->x_sm, d->M, d->D, W, K, sink, st, who);
-    }
+    const FrontSink<T, true, 4> few{*d, tab, len, n_feat};
+    if (!x_scales) return launch_of<T>(d->x, d->x_sm, d->M, d->D, W, K, few, st, who);
+    if (p || few_rows(X, W)) return launch_few(X, W, K, few, st, who);
     if constexpr (sizeof(T) == 2)
       if (d->Dh % 8 == 0) return launch_many(X, W, K, FrontSink<T, false, 8>{*d, tab, len, n_feat}, st, who);
     return launch_many(X, W, K, FrontSink<T, false, 4>{*d, tab, len, n_feat}, st, who);
