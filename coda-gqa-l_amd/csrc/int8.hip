@@ -512,7 +512,9 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // LDS.  The one barrier of a step is before its last quarter: by then every
 // wave has read all of the step, whose stage is loaded anew (step + ST) beside
 // that quarter and the next two, and the next step, whose first operands are
-// read now, has landed.  A stage holds a row's eight 16-byte pieces in the
+// read now, has landed.  Where a quarter is one product (SF = SM = 1),
+// all operands of a step are read beside the products of the one before, and
+// the barrier is at a step's start.  A stage holds a row's eight 16-byte pieces in the
 // order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
 // once (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
 // A workgroup of the largest tiles goes from tile to tile;
@@ -593,7 +595,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   // operands of quarter h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
   const uint32_t at = tile_lds(smem) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
-  i32x4 op[2][NO];
+  constexpr bool kAhead = SF == 1;  // a whole step's operands are read ahead
+  i32x4 op[kAhead ? 8 : 2][NO];
   auto read = [&](auto c, i32x4 (&o)[NO], uint32_t a) {  // operand c: SF of features, SM of tokens
     constexpr int i = decltype(c)::value;
     if constexpr (i < SF) o[i] = tile_read<i * 4096>(a + wf * (SF * 4096));
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   auto landed = [&](int n) {
     const int behind = ls - 1 - n;
     if (behind <= 0) __builtin_amdgcn_s_waitcnt(0x0f70);
-    each<ST - 2>([&](auto c) {
+    each<ST - 1>([&](auto c) {
       constexpr int v = (decltype(c)::value + 1) * NL;
       static_assert(v < 64, "vmcnt is 6 bits");
       if (behind == decltype(c)::value + 1) __builtin_amdgcn_s_waitcnt((v & 15) | (v >> 4) << 14 | 0x0f70);
@@ -655,16 +658,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
     quarter(none, one, asked, op[1], op[0], at + rat);
     ++g;
   };
+  // The same with all operands read ahead, of set now (0 or 4), the next
+  // step's to the other; loads beside the products.
+  auto step_ahead = [&](auto set) {
+    constexpr int now = decltype(set)::value, next = 4 - now, n = 4 * SF * SM, reads = 4 * NO / n + 1, loads = (NL + n - 1) / n;
+    landed(g + 1);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    rat = next_stage(rat);
+    const uint32_t then = at + rat;
+    const bool ask = lt < end;
+    each<n>([&](auto c) {
+      constexpr int p = decltype(c)::value, h = p / (SF * SM), i = p % (SF * SM) / SM, j = p % SM;
+      each<reads>([&](auto d) {
+        constexpr int o = p * reads + decltype(d)::value;
+        if constexpr (o < 4 * NO) read(std::integral_constant<int, o % NO>{}, op[next + o / NO], then ^ (32 * (o / NO)));
+      });
+      if constexpr (p * loads < NL)
+        if (ask)
+          each<loads>([&](auto d) {
+            constexpr int o = p * loads + decltype(d)::value;
+            if constexpr (o < NL) load1(std::integral_constant<int, o>{});
+          });
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[now + h][i], op[now + h][SF + j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    each<4>([&](auto h) { tile_landed(op[next + decltype(h)::value]); });
+    if (ask) loaded();
+    ++g;
+  };
   aim(place(tile));
   for (int s = 0; s < ST && lt < end; ++s) {
     each<NL>([&](auto c) { load1(c); });
     loaded();
   }
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0f70);
+  landed(0);
   __builtin_amdgcn_s_barrier();
-  each<NO>([&](auto c) { read(c, op[0], at); });
-  tile_landed(op[0]);
+  each<kAhead ? 4 : 1>([&](auto hc) {
+    constexpr int h = decltype(hc)::value;
+    each<NO>([&](auto c) { read(c, op[h], at ^ (32 * h)); });
+    tile_landed(op[h]);
+  });
   for (;;) {
     const At a = place(tile);
     float scale[3] = {0.f, 0.f, 0.f};
@@ -681,7 +716,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
       for (int j = 0; j < SM; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    for (int k = 0; k < steps; ++k) step();
+    if constexpr (kAhead) {
+      int k = 0;
+      for (; k + 1 < steps; k += 2) {
+        step_ahead(std::integral_constant<int, 0>{});
+        step_ahead(std::integral_constant<int, 4>{});
+      }
+      if (k < steps) step_ahead(std::integral_constant<int, 0>{});
+    } else {
+      for (int k = 0; k < steps; ++k) step();
+    }
     // Values pass through LDS (a wave's own part) from four features of 32
     // tokens a lane to runs of a token's features
     int le = lane;
