@@ -469,6 +469,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
                 _capturing():
             return None
         int8 = self._int8_on(x)
+        if int8 and x.shape[2] != self.embed_dim:
+            return None
         packed, rows, angles = int8 or self._packed_front_ok(x), None, None
         if not packed:
             rows = self._front_rows(x)
@@ -605,9 +607,9 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
         d = self._proj_desc(x, B, 1, cos_t, sin_t)
         int8_args = int8_tokens = int8_out = None
         if int8:
-            if D != self.embed_dim:
-                return None
             w, sw, b, ow, osw, ob = self._int8_weights()
+            if ob is not None and (ob.dtype != dt or ob.device != dev or not ob.is_contiguous()):
+                return None
             if w.device != dev:
                 raise RuntimeError(f"projection weights on {w.device}, input on {dev}")
             d.w, d.bias, int8_args = w.data_ptr(), b.data_ptr(), (sw.data_ptr(), w.stride(0), w.shape[1])

@@ -20,12 +20,13 @@ import torch
 import torch.nn as nn
 
 from . import _hip
-from .rows import _Made, _capturing
+from .rows import _Made, _capturing, _version
 
 __all__ = ["Int8Rows", "quantize_rows", "rms_norm_int8", "linear_int8"]
 
 PAD = 128        # codes of a row are stored up to a multiple of this
 MAX_ROW = 32768  # longest row that codes are made of
+MAX_STRIDE = 1 << 24  # bytes from row to row that the product's kernels span
 FLOAT_ROWS = 4  # token rows that a product's launch quantises itself
 
 
@@ -124,7 +125,7 @@ def _flat(r: Int8Rows) -> Tuple[torch.Tensor, int, torch.Tensor]:
         s = s.contiguous()
     if not c.is_contiguous():
         c = c.reshape(-1, c.shape[-1])
-        if c.stride(1) == 1 and c.stride(0) % 16 == 0 and c.data_ptr() % 16 == 0:
+        if c.stride(1) == 1 and c.stride(0) % 16 == 0 and c.stride(0) <= MAX_STRIDE and c.data_ptr() % 16 == 0:
             return c, c.stride(0), s
         c = c.contiguous()
     if c.data_ptr() % 16:
@@ -277,10 +278,11 @@ class Int8Mixin:
         shapes = dict(q_proj=(H * Dh, D), k_proj=(Hkv * Dh, D), v_proj=(Hkv * Dh, D), lambda_proj=(H, D), write_proj=(1, D),
                       o_proj=(D, H * Dh))
         lins = []
+        plain = nn.Linear.forward.__module__ == "torch.nn.modules.linear" and not nn.modules.module._has_any_global_hook()
         for n in names:
             m = self._modules[n]
-            if type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__ or \
-                    tuple(m.weight.shape) != shapes[n]:
+            if not plain or type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or \
+                    "forward" in m.__dict__ or type(m.weight) is not nn.Parameter or tuple(m.weight.shape) != shapes[n]:
                 raise RuntimeError(f"8-bit projections need {n} to be a plain nn.Linear {shapes[n]} without hooks")
             lins.append(m)
         return lins
@@ -291,7 +293,7 @@ class Int8Mixin:
         parameters are what they were."""
         lins = self._int8_linears()
         ps = [t for m in lins for t in (m.weight, m.bias) if t is not None]
-        tag = tuple((id(t), t._version, t.data_ptr(), t.dtype, t.device) for t in ps) + (self.rope_interleaved,)
+        tag = tuple((id(t), _version(t), t.data_ptr(), t.dtype, t.device) for t in ps) + (self.rope_interleaved,)
         hit = self.__dict__.get("_int8_made")
         if hit is not None and hit[0] == tag:
             hit[2].use()

@@ -15,6 +15,8 @@ namespace coda {
 static constexpr int kPad = 128;
 // the longest sum of products of int8 that int32 holds: 128 * 128 * K < 2^31
 static constexpr int kMaxK = (1 << 17) - kPad;
+// the largest row stride: a tile's rows lie within 32-bit offsets of its first
+static constexpr int64_t kMaxStride = 1 << 24;
 // elements of the longest row that the making of codes keeps in registers
 static constexpr int kMaxRow = 32768;
 
@@ -972,11 +974,12 @@ static int check_mats(const Int8Mat& X, int D, const Int8Mat& W, int K, const ch
                "%s: bad sizes rows=%d features=%d K=%d (K a multiple of %d, at most %d: int32 holds the sum)", who, X.rows,
                W.rows, K, kPad, kMaxK);
   CODA_REQUIRE(W.p && W.scales && (X.rows == 0 || X.p), "%s: null pointer", who);
-  CODA_REQUIRE((uintptr_t)W.p % 16 == 0 && W.sm % 16 == 0 && W.sm >= 0, "%s: rows of codes must lie at 16-byte addresses",
-               who);
+  const char* lie = "%s: rows of codes must lie at 16-byte addresses, %lld bytes apart at most";
+  CODA_REQUIRE((uintptr_t)W.p % 16 == 0 && W.sm % 16 == 0 && W.sm >= 0 && W.sm <= kMaxStride, lie, who,
+               (long long)kMaxStride);
   if (X.scales || X.rows == 0) {
-    CODA_REQUIRE((uintptr_t)X.p % 16 == 0 && X.sm % 16 == 0 && X.sm >= 0, "%s: rows of codes must lie at 16-byte addresses",
-                 who);
+    CODA_REQUIRE((uintptr_t)X.p % 16 == 0 && X.sm % 16 == 0 && X.sm >= 0 && X.sm <= kMaxStride, lie, who,
+                 (long long)kMaxStride);
   } else {
     CODA_REQUIRE(X.rows <= kFloatRows, "%s: %d token rows without scales (at most %d are quantised by the launch)", who,
                  X.rows, kFloatRows);

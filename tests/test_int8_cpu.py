@@ -84,7 +84,8 @@ def test_rms_norm_entry(change, error):
     (dict(K=64), "multiple of 128"), (dict(K=131072), "int32"), (dict(K=0), "sizes"), (dict(n_feat=0), "sizes"),
     (dict(M=-1), "sizes"), (dict(x=P + 1), "16-byte"), (dict(w_sm=130), "16-byte"), (dict(w=None), "null"),
     (dict(x=None), "null"), (dict(out=None), "output"), (dict(o_sm=9), "output"), (dict(dtype=3), "dtype"),
-    (dict(x_sm=-128), "16-byte"), (dict(x_scales=None, M=5), "at most 4"), (dict(x_scales=None, D=129), "129 elements"),
+    (dict(x_sm=-128), "16-byte"), (dict(x_sm=(1 << 24) + 16), "apart at most"), (dict(w_sm=1 << 25), "apart at most"),
+    (dict(x_scales=None, M=5), "at most 4"), (dict(x_scales=None, D=129), "129 elements"),
     (dict(x_scales=None, D=0), "0 elements"), (dict(x_scales=None, x=None), "null"),
 ])
 def test_linear_entry(change, error):
@@ -128,3 +129,46 @@ def test_project_entry_tables(dim, params, error):
     L = _hip.lib()
     assert L.coda_project_int8(d, P, P, 128, 128, p, None) == 1
     assert error in L.coda_last_error().decode()
+
+
+def _layer():
+    m = coda_gqa_l.CoDAGQA(embed_dim=128, num_heads=4, num_kv_heads=2).bfloat16().eval()
+    return m.use_int8_projections()
+
+
+class _Mine(torch.nn.Linear):
+    pass
+
+
+class _Weight(torch.nn.Parameter):
+    pass
+
+
+@pytest.mark.parametrize("change", [
+    lambda m: m.q_proj.register_forward_hook(lambda *a: None),
+    lambda m: m.o_proj.register_forward_pre_hook(lambda *a: None),
+    lambda m: setattr(m.k_proj, "forward", lambda x: x),
+    lambda m: setattr(m, "v_proj", _Mine(128, 64)),
+    lambda m: setattr(m.lambda_proj, "weight", _Weight(m.lambda_proj.weight.detach().clone())),
+    lambda m: setattr(m, "q_proj", torch.nn.Linear(128, 64, bias=False)),
+    lambda m: setattr(m, "o_proj", torch.nn.Linear(64, 128, bias=False)),
+    lambda m: torch.nn.utils.parametrize.register_parametrization(m.q_proj, "weight", torch.nn.Identity()),
+])
+def test_only_plain_projections(change):
+    import torch.nn.utils.parametrize  # noqa: F401
+    m = _layer()
+    assert len(m._int8_linears()) == 5
+    change(m)
+    with pytest.raises(RuntimeError, match="plain nn.Linear"):
+        m._int8_linears()
+
+
+def test_hooks_on_every_module():
+    m = _layer()
+    h = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    try:
+        with pytest.raises(RuntimeError, match="plain nn.Linear"):
+            m._int8_linears()
+    finally:
+        h.remove()
+    assert len(m._int8_linears()) == 5

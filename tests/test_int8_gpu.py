@@ -216,7 +216,7 @@ def test_longest_sum(M):
     assert (y[:, ::2] == want).all() and (y[:, 1::2] == -want).all()
 
 
-@pytest.mark.parametrize("M", [2, 100, 700])
+@pytest.mark.parametrize("M", [2, 100, 118, 700])
 def test_codes_of_any_layout(M):
     """Rows with gaps, rows off 16 bytes, one row for all tokens, leading
     dimensions: as dense codes."""
@@ -230,6 +230,10 @@ def test_codes_of_any_layout(M):
     for c in (gap, off, odd):
         assert torch.equal(linear_int8(Int8Rows(c, sa, K, torch.bfloat16), w), dense)
     wide = torch.empty(N, 2 * K, dtype=torch.int8, device=DEV)[:, K:].copy_(b)
+    far = torch.empty(M, 1 << 15, K, dtype=torch.int8, device=DEV)[:, 7].copy_(a) if M < 120 else a  # 16 MiB apart
+    further = torch.empty(M, (1 << 15) + 1, K, dtype=torch.int8, device=DEV)[:, 7].copy_(a) if M < 120 else a
+    for c in (far, further):
+        assert torch.equal(linear_int8(Int8Rows(c, sa, K, torch.bfloat16), w), dense)
     scales = torch.stack([sb, sb], 1)[:, 0]
     assert torch.equal(linear_int8(Int8Rows(a, sa, K, torch.bfloat16), Int8Rows(wide, scales, K, torch.bfloat16)), dense)
     same = linear_int8(Int8Rows(a[:1].expand(M, K), sa[:1].expand(M), K, torch.bfloat16), w)

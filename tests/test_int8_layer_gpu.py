@@ -257,6 +257,17 @@ def test_refused():
     m.use_int8_projections()
     with pytest.raises(RuntimeError, match="not \\(B, L, 512\\)"):
         m._front_int8(quantize_rows(x[..., :500]), 0)
+    # a steady state, then tokens of another width, or an o_proj bias of another type
+    m.prefill_chunked(_rand(_gen(2), 1, 60, 512, dtype=torch.bfloat16), st, block_size=32)
+    m.step(x[:, :1], st)
+    for bad in (x[:, :1, :500], quantize_rows(x[:, :1, :500]), torch.cat([x[:, :1]] * 2, 2)):
+        with pytest.raises(RuntimeError, match="not \\(B, L, 512\\)"):
+            m.step(bad, st)
+    m.o_proj.bias = nn.Parameter(torch.zeros(512, device=DEV))
+    with pytest.raises(RuntimeError, match="bias"):
+        m.step(x[:, :1], st)
+    m.o_proj.bias = None
+    m.step(x[:, :1], st)
     h = m.k_proj.register_forward_hook(lambda *a: None)
     with pytest.raises(RuntimeError, match="k_proj to be a plain"):
         m.prefill_chunked(x, st)
