@@ -7,6 +7,7 @@
 // product runs over whole 128-byte steps and has no ragged end.
 #include "rows.h"
 
+#include <algorithm>
 #include <climits>
 #include <utility>
 
@@ -480,6 +481,7 @@ __device__ __forceinline__ i32x4 tile_read(uint32_t addr) {
 template <int N>
 __device__ __forceinline__ void tile_landed(i32x4 (&a)[N]) {
   if constexpr (N == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]));
+  if constexpr (N == 3) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]));
   if constexpr (N == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
   if constexpr (N == 6)
     asm volatile("s_waitcnt lgkmcnt(0)"
@@ -514,7 +516,7 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // LDS.  The one barrier of a step is before its last quarter: by then every
 // wave has read all of the step, whose stage is loaded anew (step + ST) beside
 // that quarter and the next two, and the next step, whose first operands are
-// read now, has landed.  Where a quarter is one product (SF = SM = 1),
+// read now, has landed.  Where a quarter is a product or two (SF = 1),
 // all operands of a step are read beside the products of the one before, and
 // the barrier is at a step's start.  A stage holds a row's eight 16-byte pieces in the
 // order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
@@ -932,28 +934,29 @@ static int launch_few(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sin
 static int64_t tiles_of(const Int8Mat& X, const Int8Mat& W, int f, int m) {
   return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m);
 }
-// Whether the row kernels or the smallest tiles: up to 64 rows the former, up
-// to 128 where the tiles do not go round in one (us, rows and tiles: 17 x 4096
-// x 6177 11.5 and 14.2, 64 x 4096 x 4096 10.0 and 13.6, 64 x 4096 x 6177 14.6
-// both, 128 x 4096 x 6177 19.2 and 14.9, 128 x 8192 x 8192 32.0 and 27.1, 128
-// x 8192 x 10305, 322 tiles, 38.1 and 40.9).
-static bool few_rows(const Int8Mat& X, const Int8Mat& W) {
-  return X.rows <= 64 || (X.rows <= kFewRows && tiles_of(X, W, 64, 64) > device_cus());
-}
+// The row kernels or tiles: up to 64 rows the former (us, rows and tiles: 17 x
+// 4096 x 6177 11.5 and 14.2, 64 x 4096 x 4096 10.0 and 12.9, 64 x 8192 x 8192
+// 24.7 and 26.8, 64 x 4096 x 6177 14.6 and 13.7, 128 x 4096 x 6177 19.2 and
+// 13.7, 128 x 8192 x 8192 32.0 and 26.4, 128 x 8192 x 10305 38.1 and 33.0).
+static bool few_rows(const Int8Mat& X) { return X.rows <= 64; }
 // The tile by the time that its rounds take, us a round of one tile (64 x 64:
 // two) a CU at K = 4096.  Measured, 256 x 256 | 256 x 128 | 128 x 128 | 64 x
-// 64: 1999 x 4096 x 4096 55 41 50 75, 1999 x 4096 x 6177 58 68 81 107, 1000 x
-// 4096 x 4096 52 31 24 38, 300 x 4096 x 6177 - - 20 21, 500 x 2048 x 3105 - -
-// 12.5 11.3, 4096 x 4096 x 6177 112 130 - -, 2000 x 1024 x 1024 - - 9.3 8.1.
+// 128 | 64 x 64 (features x tokens): 1999 x 4096 x 4096 55 41 50 - 75, 1999 x
+// 4096 x 6177 58 68 81 - 107, 1000 x 4096 x 4096 52 31 24 35 38, 300 x 4096 x
+// 6177 - 37 20 32 21, 500 x 2048 x 3105 - 19 12.5 10.6 10.8, 128 x 8192 x
+// 10305 - - 43 33 41, 128 x 8192 x 8192 - - 42 32 26, 4096 x 4096 x 6177 112
+// 130 157 - -, 2000 x 1024 x 1024 - - 9.3 - 8.1.
 template <typename Sink>
 static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
   const int64_t cus = device_cus(), n1 = tiles_of(X, W, 64, 64);
   const auto rounds = [&](int f, int m) { return (tiles_of(X, W, f, m) + cus - 1) / cus; };
   const int64_t t44 = 56 * rounds(256, 256), t42 = 39 * rounds(256, 128), t22 = 23 * rounds(128, 128);
-  const int64_t t11 = n1 <= cus ? 15 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
-  if (t44 <= t42 && t44 <= t22 && t44 <= t11) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
-  if (t42 <= t22 && t42 <= t11) return launch_tile<4, 2, 3>(X, W, K, sink, st, who);
-  if (t22 <= t11) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
+  const int64_t t12 = 17 * rounds(64, 128), t11 = n1 <= cus ? 15 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
+  const int64_t least = std::min({t44, t42, t22, t12, t11});
+  if (t44 == least) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
+  if (t42 == least) return launch_tile<4, 2, 3>(X, W, K, sink, st, who);
+  if (t22 == least) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
+  if (t12 == least) return launch_tile<1, 2, 4>(X, W, K, sink, st, who);
   return launch_tile<1, 1, 4>(X, W, K, sink, st, who);
 }
 
@@ -1051,8 +1054,8 @@ extern "C" int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const fl
     typedef decltype(t) T;
     const LinearSink<T> sink{(T*)out, (const T*)bias, o_sm, n_feat};
     return !x_scales       ? launch_of<T>(x, x_sm, M, D, W, K, sink, st, who)
-           : few_rows(X, W) ? launch_few(X, W, K, sink, st, who)
-                            : launch_many(X, W, K, sink, st, who);
+           : few_rows(X) ? launch_few(X, W, K, sink, st, who)
+                         : launch_many(X, W, K, sink, st, who);
   };
   return dtype == CODA_F32 ? run(float{}) : dtype == CODA_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
@@ -1092,7 +1095,10 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
     typedef decltype(t) T;
     const FrontSink<T, true, 4> few{*d, tab, len, n_feat};
     if (!x_scales) return launch_of<T>(d->x, d->x_sm, d->M, d->D, W, K, few, st, who);
-    if (p || few_rows(X, W)) return launch_few(X, W, K, few, st, who);
+    // (tiles that do not go round in one wait for their tokens' RoPE rows too
+    // often: 128 x 8192 x 10305 37.4 us against 33.8)
+    if (p || few_rows(X) || (d->M <= kFewRows && tiles_of(X, W, 64, 64) > device_cus()))
+      return launch_few(X, W, K, few, st, who);
     if constexpr (sizeof(T) == 2)
       if (d->Dh % 8 == 0) return launch_many(X, W, K, FrontSink<T, false, 8>{*d, tab, len, n_feat}, st, who);
     return launch_many(X, W, K, FrontSink<T, false, 4>{*d, tab, len, n_feat}, st, who);
