@@ -375,6 +375,13 @@ struct FrontSink {
     if (f < Fq + 2 * Fk) return Lane{0, 0, (T*)d.v + (f - Fq - Fk), d.v_sm};
     return Lane{2, f, nullptr, 0};
   }
+  // Of 16-bit values by the hardware's exponential and reciprocal, off by some
+  // 2^-22 where the result is rounded to 2^-9 (the lambdas of a tile are few
+  // lanes' work and hold up the whole launch: 35 instructions against 4).
+  static __device__ __forceinline__ float sigmoid(float x) {
+    if constexpr (sizeof(T) == 4) return proj_sigmoid(x);
+    else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+  }
   // a row's runs of n T's: at 8-byte addresses at least (the entry's checks)
   template <int n>
   static __device__ __forceinline__ void st(T* p, const Feats<T, n>& v) {
@@ -439,7 +446,7 @@ struct FrontSink {
           const int f = l.c + e;
           const int64_t mr = m + r * step;
           if (f >= n_feat || mr >= rows) continue;
-          const float sg = E::rnd(proj_sigmoid(E::ld(v[r].v[e])));
+          const float sg = E::rnd(sigmoid(E::ld(v[r].v[e])));
           if (f < o_g) ((T*)d.lam)[mr * d.lam_sm + (f - o_l)] = E::st(sg);
           else d.g[mr] = sg;
         }
