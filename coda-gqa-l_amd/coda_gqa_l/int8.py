@@ -84,9 +84,13 @@ class Int8Rows:
         dtype = self.dtype if dtype is None else dtype
         code = _hip.dtype_code(dtype)
         codes, sm, scales = _flat(self)
-        out = torch.empty(self.shape, dtype=dtype, device=codes.device)
-        _call(_hip.lib().coda_dequantize_rows, codes, code, codes.data_ptr(), sm, scales.data_ptr(), scales.numel(),
-              self.cols, out.data_ptr(), self.cols)
+        cols = self.cols
+        if cols == sm and codes is self.codes:
+            out = torch.empty_like(codes, dtype=dtype)
+        else:
+            out = torch.empty(self.shape, dtype=dtype, device=codes.device)
+        _call(_hip.lib().coda_dequantize_rows, codes.get_device(), code, codes.data_ptr(), sm, scales.data_ptr(),
+              scales.numel(), cols, out.data_ptr(), cols)
         return out
 
 
@@ -102,10 +106,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(fn, t: torch.Tensor, *args) -> None:
-    """A library call on t's device, whichever is current, and its current
+def _call(fn, index: int, *args) -> None:
+    """A library call on device `index`, whichever is current, and its current
     stream."""
-    index = t.get_device()
     if index == torch.cuda.current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -119,18 +122,14 @@ def _flat(r: Int8Rows) -> Tuple[torch.Tensor, int, torch.Tensor]:
     """(codes whose rows lie at 16-byte addresses, bytes from one to the next,
     scales without gaps), copied only where they do not lie so."""
     c, s = r.codes, r.scales
-    if not c.is_cuda:
-        _hip.require_device(c, s)
-    if not s.is_contiguous():
-        s = s.contiguous()
-    if not c.is_contiguous():
-        c = c.reshape(-1, c.shape[-1])
-        if c.stride(1) == 1 and c.stride(0) % 16 == 0 and c.stride(0) <= MAX_STRIDE and c.data_ptr() % 16 == 0:
-            return c, c.stride(0), s
-        c = c.contiguous()
-    if c.data_ptr() % 16:
-        c = c.clone()
-    return c, c.shape[-1], s
+    if c.is_contiguous() and s.is_contiguous() and not c.data_ptr() % 16 and c.is_cuda:
+        return c, c.shape[-1], s
+    _hip.require_device(c, s)
+    s, P = s.contiguous(), c.shape[-1]
+    c = c.reshape(-1, P)
+    if c.stride(1) == 1 and c.stride(0) % 16 == 0 and c.stride(0) <= MAX_STRIDE and c.data_ptr() % 16 == 0:
+        return c, c.stride(0), s
+    return c.clone(memory_format=torch.contiguous_format), P, s
 
 
 def _rows_of(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -170,7 +169,7 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     code = _hip.dtype_code(dt)
     x2, sm = _rows_of(x)
     codes, scales, P = _new_rows(x, D)
-    _call(_hip.lib().coda_quantize_rows, x, code, x2.data_ptr(), sm, scales.numel(), D, codes.data_ptr(), P,
+    _call(_hip.lib().coda_quantize_rows, x.get_device(), code, x2.data_ptr(), sm, scales.numel(), D, codes.data_ptr(), P,
           scales.data_ptr())
     return _made(codes, scales, D, dt)
 
@@ -182,17 +181,11 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     rounded to x's type, and (rows, s) is returned: s is the residual of the
     next sublayer.  x, weight (D,) and residual share their type; D at most
     32768."""
-    D = _check_input(x, "rms_norm_int8")
-    dt = x.dtype
+    D, dt, index = _check_input(x, "rms_norm_int8"), x.dtype, x.get_device()
     code = _hip.dtype_code(dt)
-    if weight.shape != (D,):
-        raise RuntimeError(f"rms_norm_int8: weight {tuple(weight.shape)}, expected ({D},)")
-    if residual is not None and residual.shape != x.shape:
-        raise RuntimeError(f"rms_norm_int8: residual {tuple(residual.shape)} is not x's shape {tuple(x.shape)}")
-    if weight.dtype is not dt or weight.device != x.device:
-        raise RuntimeError(f"rms_norm_int8: weight is {weight.dtype} on {weight.device}, x {dt} on {x.device}")
-    if residual is not None and (residual.dtype is not dt or residual.device != x.device):
-        raise RuntimeError(f"rms_norm_int8: residual is {residual.dtype} on {residual.device}, x {dt} on {x.device}")
+    if weight.dtype is not dt or weight.get_device() != index or weight.shape != (D,):
+        raise RuntimeError(f"rms_norm_int8: weight is {tuple(weight.shape)} {weight.dtype} on {weight.device}, expected "
+                           f"({D},) {dt} on {x.device}")
     if not eps >= 0:
         raise RuntimeError(f"rms_norm_int8: eps={eps} is negative")
     x2, sm = _rows_of(x)
@@ -200,13 +193,16 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     codes, scales, P = _new_rows(x, D)
     fn = _hip.lib().coda_rms_norm_int8
     if residual is None:
-        _call(fn, x, code, x2.data_ptr(), sm, None, 0, w.data_ptr(), scales.numel(), D, float(eps), None, 0,
-              codes.data_ptr(), P, scales.data_ptr())
+        _call(fn, index, code, x2.data_ptr(), sm, None, 0, w.data_ptr(), scales.numel(), D, eps, None, 0, codes.data_ptr(),
+              P, scales.data_ptr())
         return _made(codes, scales, D, dt)
+    if residual.dtype is not dt or residual.get_device() != index or residual.shape != x.shape:
+        raise RuntimeError(f"rms_norm_int8: residual is {tuple(residual.shape)} {residual.dtype} on {residual.device}, x "
+                           f"{tuple(x.shape)} {dt} on {x.device}")
     r2, rm = _rows_of(residual)
     out = torch.empty_like(x2) if x2 is x else torch.empty(x.shape, dtype=dt, device=x.device)
-    _call(fn, x, code, x2.data_ptr(), sm, r2.data_ptr(), rm, w.data_ptr(), scales.numel(), D, float(eps),
-          out.data_ptr(), D, codes.data_ptr(), P, scales.data_ptr())
+    _call(fn, index, code, x2.data_ptr(), sm, r2.data_ptr(), rm, w.data_ptr(), scales.numel(), D, eps, out.data_ptr(), D,
+          codes.data_ptr(), P, scales.data_ptr())
     return _made(codes, scales, D, dt), out
 
 
@@ -216,32 +212,35 @@ def linear_int8(x: Union[Int8Rows, torch.Tensor], weight: Int8Rows, bias: Option
     (N,), rounded once to x's type.  K at most 130944.  A tensor x is
     quantised by rows first (quantize_rows; K at most 32768), up to 4 rows on
     the product's own way through the weights: the same bits."""
-    if not isinstance(weight, Int8Rows) or not isinstance(x, (Int8Rows, torch.Tensor)):
+    rows = isinstance(x, Int8Rows)
+    if not isinstance(weight, Int8Rows) or not rows and not isinstance(x, torch.Tensor):
         raise TypeError("linear_int8 takes a tensor or Int8Rows, and a weight in Int8Rows (quantize_rows makes them)")
-    wc, dt, shape = weight.codes, x.dtype, x.shape
-    if wc.dim() != 2 or not shape or weight.cols != shape[-1] or wc.shape[0] == 0:
-        raise RuntimeError(f"linear_int8: weight {tuple(weight.shape)} does not fit x {tuple(shape)}")
-    N, P = wc.shape
     b, bm, sb = _flat(weight)
-    sa = None
-    if not isinstance(x, Int8Rows):
-        K = _check_input(x, "linear_int8")
-        M = x.numel() // K
+    N, P = sb.numel(), weight.codes.shape[-1]
+    if rows:
+        K, lead = x.cols, x.scales.shape
+        a, am, sa = _flat(x)
+        M, sp = sa.numel(), sa.data_ptr()
+    else:
+        K, lead = _check_input(x, "linear_int8"), x.shape[:-1]
+        M, sp = x.numel() // K, None
         if M <= FLOAT_ROWS:
             a, am = _rows_of(x)
         else:
             x = quantize_rows(x)
-    if isinstance(x, Int8Rows):
-        a, am, sa = _flat(x)
-        M = sa.numel()
-    dev = a.device
-    if b.device != dev or bias is not None and (bias.device != dev or bias.dtype is not dt or bias.shape != (N,)):
+            a, am, sa = x.codes, P, x.scales
+            sp = sa.data_ptr()
+    if weight.cols != K or weight.scales.dim() != 1 or not N:
+        raise RuntimeError(f"linear_int8: weight {tuple(weight.shape)} does not fit x {tuple(x.shape)}")
+    dt, index = x.dtype, a.get_device()
+    if b.get_device() != index or bias is not None and (bias.get_device() != index or bias.dtype is not dt or
+                                                        bias.shape != (N,)):
         raise RuntimeError("linear_int8: weight and bias must be on x's device, bias (N,) of x's type")
     if bias is not None:
         bias = bias.contiguous()
-    out = torch.empty((*shape[:-1], N), dtype=dt, device=dev)
-    _call(_hip.lib().coda_linear_int8, a, _hip.dtype_code(dt), a.data_ptr(), am, None if sa is None else sa.data_ptr(), M,
-          shape[-1], b.data_ptr(), bm, sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
+    out = torch.empty((*lead, N), dtype=dt, device=a.device)
+    _call(_hip.lib().coda_linear_int8, index, _hip.dtype_code(dt), a.data_ptr(), am, sp, M, K, b.data_ptr(), bm,
+          sb.data_ptr(), N, P, None if bias is None else bias.data_ptr(), out.data_ptr(), N)
     return out
 
 
@@ -331,7 +330,7 @@ class Int8Mixin:
             x = quantize_rows(x)
         xs, d.x_sm, scales = _flat(x) if isinstance(x, Int8Rows) else (*_rows_of(x), None)
         d.x, d.w, d.bias = xs.data_ptr(), w.data_ptr(), bias.data_ptr()
-        _call(_hip.lib().coda_project_int8, xs, d, _hip.ptr(scales), sw.data_ptr(), w.stride(0), w.shape[1], p)
+        _call(_hip.lib().coda_project_int8, xs.get_device(), d, _hip.ptr(scales), sw.data_ptr(), w.stride(0), w.shape[1], p)
         return xs, scales
 
     def _front_int8(self, x, p0: int):
