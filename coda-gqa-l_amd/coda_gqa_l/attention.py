@@ -469,8 +469,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
                 _capturing():
             return None
         int8 = self._int8_on(x)
-        if int8 and x.shape[2] != self.embed_dim:
-            return None
+        if int8 and (x.shape[2] != self.embed_dim or not self._int8_still_plain()):
+            return None  # (the general path refuses them)
         packed, rows, angles = int8 or self._packed_front_ok(x), None, None
         if not packed:
             rows = self._front_rows(x)
@@ -482,8 +482,8 @@ class CoDAGQALandmarkPerf2(MemoryBankMixin, Int8Mixin, RowsMixin, nn.Module):
         vers = tuple(-1 if t is None else t._version for t in ts)
         pvers = self._param_key()
         B, stream = x.shape[0], _hip.stream_of(x)
-        if fp is None or fp["int8"] != int8 or fp["st"] is not st or fp["vers"] != vers or fp["pvers"] != pvers or fp["B"] != B or \
-                fp["packed"] != packed or fp["dtype"] is not x.dtype or fp["stream"] != stream or \
+        if fp is None or fp["int8"] != int8 or fp["st"] is not st or fp["vers"] != vers or fp["pvers"] != pvers or \
+                fp["B"] != B or fp["packed"] != packed or fp["dtype"] is not x.dtype or fp["stream"] != stream or \
                 fp["ptrs"] != tuple(-1 if t is None else t.data_ptr() for t in ts) or fp["dev"] != x.device:
             fp = self._build_step_fast(x, st, ts, vers, pvers, packed, int8)
             if fp is None:

@@ -8,8 +8,9 @@ the product of two sets of them.
   Int8Rows       - the codes and scales that these hand on
 
 The layers run their projections on them after use_int8_projections()
-(Int8Mixin), and take Int8Rows in place of a tensor.  Inference only: no output carries a gradient.  Errors surface
-as RuntimeError, like those of the other operators.
+(Int8Mixin), and take Int8Rows in place of a tensor.  Inference only: no output
+carries a gradient.  Errors surface as RuntimeError, like those of the other
+operators.
 """
 
 from __future__ import annotations
@@ -124,6 +125,8 @@ def _flat(r: Int8Rows) -> Tuple[torch.Tensor, int, torch.Tensor]:
     c, s = r.codes, r.scales
     if c.is_contiguous() and s.is_contiguous() and not c.data_ptr() % 16 and c.is_cuda:
         return c, c.shape[-1], s
+    if s.numel() >= 1 << 31:
+        raise RuntimeError(f"Int8Rows: {s.numel()} rows, a call takes less than 2^31")
     _hip.require_device(c, s)
     s, P = s.contiguous(), c.shape[-1]
     c = c.reshape(-1, P)
@@ -271,17 +274,30 @@ class Int8Mixin:
             return True
         return self.int8_projections
 
+    def _int8_names(self) -> tuple:
+        return ("q_proj", "k_proj", "v_proj", "lambda_proj") + (("write_proj",) if self._has_gate() else ()) + ("o_proj",)
+
+    def _int8_plain(self, name: str) -> bool:
+        """Whether a projection's module does what nn.Linear does, and no more."""
+        m = self._modules[name]
+        return type(m) is nn.Linear and not (m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__)
+
+    def _int8_still_plain(self) -> bool:
+        """The part of _int8_linears that a cached step does not see in the
+        parameters' identities and versions."""
+        return nn.Linear.forward.__module__ == "torch.nn.modules.linear" and \
+            not nn.modules.module._has_any_global_hook() and all(map(self._int8_plain, self._int8_names()))
+
     def _int8_linears(self) -> list:
-        names = ("q_proj", "k_proj", "v_proj", "lambda_proj") + (("write_proj",) if self._has_gate() else ()) + ("o_proj",)
         H, Hkv, Dh, D = self.num_heads, self.num_kv_heads, self.head_dim, self.embed_dim
         shapes = dict(q_proj=(H * Dh, D), k_proj=(Hkv * Dh, D), v_proj=(Hkv * Dh, D), lambda_proj=(H, D), write_proj=(1, D),
                       o_proj=(D, H * Dh))
         lins = []
         plain = nn.Linear.forward.__module__ == "torch.nn.modules.linear" and not nn.modules.module._has_any_global_hook()
-        for n in names:
+        for n in self._int8_names():
             m = self._modules[n]
-            if not plain or type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or \
-                    "forward" in m.__dict__ or type(m.weight) is not nn.Parameter or tuple(m.weight.shape) != shapes[n]:
+            if not plain or not self._int8_plain(n) or type(m.weight) is not nn.Parameter or \
+                    tuple(m.weight.shape) != shapes[n]:
                 raise RuntimeError(f"8-bit projections need {n} to be a plain nn.Linear {shapes[n]} without hooks")
             lins.append(m)
         return lins

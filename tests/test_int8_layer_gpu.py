@@ -280,6 +280,31 @@ def test_refused():
         half._front_int8(x.half(), 0)
 
 
+@torch.no_grad()
+@pytest.mark.parametrize("name", ["q_proj", "write_proj", "o_proj"])
+def test_hooks_between_steps(name):
+    """A hook, or a forward of its own, that a projection gets once steps run
+    from descriptors is refused, and steps go on without it."""
+    m = _bounded()
+    st = _state(m, 1, torch.bfloat16)
+    g = _gen(3)
+    m.prefill_chunked(_rand(g, 1, 60, 512, dtype=torch.bfloat16), st, block_size=32)
+    x = _rand(g, 1, 1, 512, dtype=torch.bfloat16)
+    m.step(x, st)
+    m.step(x, st)
+    lin = getattr(m, name)
+    for add, remove in ((lambda: lin.register_forward_hook(lambda *a: None), lambda h: h.remove()),
+                        (lambda: lin.register_forward_pre_hook(lambda *a: None), lambda h: h.remove()),
+                        (lambda: setattr(lin, "forward", lambda t: t), lambda h: delattr(lin, "forward"))):
+        pos = int(st.pos)
+        h = add()
+        with pytest.raises(RuntimeError, match=name + " to be a plain"):
+            m.step(x, st)
+        assert int(st.pos) == pos
+        remove(h)
+        m.step(x, st)
+
+
 # ---------------------------------------------------------------- unbounded layer
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,L,past,causal", [(1, 1, 0, True), (2, 65, 0, True), (1, 300, 0, False), (2, 3, 50, False),
