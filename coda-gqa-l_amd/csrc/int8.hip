@@ -20,6 +20,10 @@ static constexpr int kMaxK = (1 << 17) - kPad;
 static constexpr int64_t kMaxStride = 1 << 24;
 // elements of the longest row that the making of codes keeps in registers
 static constexpr int kMaxRow = 32768;
+// rows of a launch of a row a workgroup (a grid has less than 2^32 threads)
+static constexpr int64_t kLaunchRows = 1 << 21;
+// rows of a product's operand (their numbers, up to a whole tile, are 32 bits)
+static constexpr int kMaxRows = 1 << 30;
 
 // ------------------------------------------------------------ making codes
 __device__ __forceinline__ double wave_reduce(double v, bool max) {
@@ -118,7 +122,11 @@ using PlainR = typename std::conditional<sizeof(T) == 2, float, double>::type;
 // NaN (its weight's count too) gets scale NaN and codes 0; a row of zeros
 // scale 0.
 // TPR threads keep a row in registers (IT runs of 8 elements each) between
-// the row's maximum and its codes, so that memory is read once.
+// the row's maximum and its codes, so that memory is read once.  It is bound
+// by memory where rows are many: 16384 x 8192 bf16 with a residual 164-180 us
+// (5.2-5.7 TB/s), plain 76 us (5.3); 1 x 4096 with a residual 3.2 us, a
+// launch.  A wave for a row of up to 1024 elements needs no barrier; longer
+// ones share it, 16 elements a thread (1024 threads: up to 32).
 template <typename T, bool NORM, bool RES, int TPR, int IT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void codes_kernel(
     const T* __restrict__ x, int64_t x_sm, const T* __restrict__ res, int64_t r_sm, const T* __restrict__ w, int rows,
@@ -211,9 +219,15 @@ template <typename T, bool NORM, bool RES, int TPR, int IT>
 static int launch_codes(const T* x, int64_t x_sm, const T* res, int64_t r_sm, const T* w, int rows, int D, float eps,
                         T* sum_out, int64_t s_sm, int8_t* codes, int64_t c_sm, float* scales, hipStream_t st) {
   constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-  hipLaunchKernelGGL((codes_kernel<T, NORM, RES, TPR, IT>), dim3((unsigned)(((int64_t)rows + RPB - 1) / RPB)), dim3(NT),
-                     0, st, x, x_sm, res, r_sm, w, rows, D, eps, sum_out, s_sm, codes, c_sm, scales);
-  return check_launch("codes_kernel");
+  for (int64_t r = 0; r < rows; r += kLaunchRows) {
+    const int n = (int)std::min(kLaunchRows, rows - r);
+    hipLaunchKernelGGL((codes_kernel<T, NORM, RES, TPR, IT>), dim3((n + RPB - 1) / RPB), dim3(NT), 0, st, x + r * x_sm, x_sm,
+                       RES ? res + r * r_sm : res, r_sm, w, n, D, eps, RES ? sum_out + r * s_sm : sum_out, s_sm,
+                       codes + r * c_sm, c_sm, scales + r);
+    const int rc = check_launch("codes_kernel");
+    if (rc) return rc;
+  }
+  return CODA_OK;
 }
 
 // threads and runs of a row of D elements (up to a multiple of 128)
@@ -235,7 +249,8 @@ static int run_codes(const void* x, int64_t x_sm, const void* res, int64_t r_sm,
 }
 
 // values of codes: out = code * scale, one rounding to T.  TPR threads a row
-// and workgroup, 8 codes each; out rows of any element address.
+// and workgroup, 8 codes each; out rows of any element address.  Bound by
+// memory: 16384 x 8192 to bf16 70-74 us (5.4-5.7 TB/s).
 template <typename T, int TPR>
 __global__ __launch_bounds__(256) void values_kernel(const int8_t* __restrict__ codes, int64_t c_sm,
                                                      const float* __restrict__ scales, int rows, int D,
@@ -257,13 +272,19 @@ template <typename T>
 static int run_values(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, void* out, int64_t o_sm,
                       hipStream_t st) {
   // (a row of up to 512 elements leaves most of 256 threads idle)
-  if (D <= 512)
-    hipLaunchKernelGGL((values_kernel<T, 64>), dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(256), 0, st, codes, c_sm,
-                       scales, rows, D, (T*)out, o_sm);
-  else
-    hipLaunchKernelGGL((values_kernel<T, 256>), dim3((unsigned)rows, (unsigned)((D + 2047) / 2048)), dim3(256), 0, st,
-                       codes, c_sm, scales, rows, D, (T*)out, o_sm);
-  return check_launch("values_kernel");
+  for (int64_t r = 0; r < rows; r += kLaunchRows) {
+    const int n = (int)std::min(kLaunchRows, rows - r);
+    const int8_t* c = codes + r * c_sm;
+    T* o = (T*)out + r * o_sm;
+    if (D <= 512)
+      hipLaunchKernelGGL((values_kernel<T, 64>), dim3((n + 3) / 4), dim3(256), 0, st, c, c_sm, scales + r, n, D, o, o_sm);
+    else
+      hipLaunchKernelGGL((values_kernel<T, 256>), dim3(n, (D + 2047) / 2048), dim3(256), 0, st, c, c_sm, scales + r, n, D, o,
+                         o_sm);
+    const int rc = check_launch("values_kernel");
+    if (rc) return rc;
+  }
+  return CODA_OK;
 }
 
 // ------------------------------------------------------------ product
@@ -528,10 +549,13 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // the barrier is at a step's start.  A stage holds a row's eight 16-byte pieces in the
 // order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
 // once (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
-// A workgroup of the largest tiles goes from tile to tile;
-// the stages run on over the border, so that the next tile's first steps are
-// in LDS when this one's values have been written, and the writes are on
-// their way while its products run.
+// A workgroup of the largest tiles goes from tile to tile; the stages run on
+// over the border, so that the next tile's first steps are in LDS when this
+// one's values have been written, and the writes are on their way while its
+// products run.  Those are bound by the matrix pipe, whose clock falls to 1.25
+// to 1.6 GHz under it: 16384 x 8192 x 8192 880-900 us = 2440-2500 TOP/s, 32768
+// x 4096 x 6177 767 us; the smaller ones by what L2 and LDS deliver beside few
+// products: 1999 x 4096 x 4096 41 us, 128 x 8192 x 8192 26.
 template <int SF, int SM, int ST, typename T>
 struct TileLds {
   static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
@@ -795,7 +819,8 @@ static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   typedef TileLds<SF, SM, ST, typename Sink::Out> L;
   const int64_t ntf = ((int64_t)W.rows + 64 * SF - 1) / (64 * SF), ntm = ((int64_t)X.rows + 64 * SM - 1) / (64 * SM);
   const int64_t n = ntf * ntm;
-  if (n > INT_MAX / 8) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
+  // (a grid has less than 2^32 threads; a walk's tiles are counted in 32 bits)
+  if (n >= (L::kWalk ? INT_MAX / 8 : 1 << 24)) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
   const int rc = lds_limit<int8_tile<SF, SM, ST, Sink>>(L::kBytes, who);
   if (rc) return rc;
   const int64_t grid = L::kWalk && n > device_cus() ? device_cus() : n;
@@ -983,6 +1008,8 @@ static int check_mats(const Int8Mat& X, int D, const Int8Mat& W, int K, const ch
   CODA_REQUIRE(X.rows >= 0 && W.rows > 0 && K > 0 && K % kPad == 0 && K <= kMaxK,
                "%s: bad sizes rows=%d features=%d K=%d (K a multiple of %d, at most %d: int32 holds the sum)", who, X.rows,
                W.rows, K, kPad, kMaxK);
+  if (X.rows > kMaxRows || W.rows > kMaxRows)
+    return fail(CODA_EUNSUP, "%s: %d rows times %d (at most 2^30)", who, X.rows, W.rows);
   CODA_REQUIRE(W.p && W.scales && (X.rows == 0 || X.p), "%s: null pointer", who);
   const char* lie = "%s: rows of codes must lie at 16-byte addresses, %lld bytes apart at most";
   CODA_REQUIRE((uintptr_t)W.p % 16 == 0 && W.sm % 16 == 0 && W.sm >= 0 && W.sm <= kMaxStride, lie, who,
@@ -1060,9 +1087,8 @@ extern "C" int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const fl
   const auto run = [&](auto t) {
     typedef decltype(t) T;
     const LinearSink<T> sink{(T*)out, (const T*)bias, o_sm, n_feat};
-    return !x_scales       ? launch_of<T>(x, x_sm, M, D, W, K, sink, st, who)
-           : few_rows(X) ? launch_few(X, W, K, sink, st, who)
-                         : launch_many(X, W, K, sink, st, who);
+    if (!x_scales) return launch_of<T>(x, x_sm, M, D, W, K, sink, st, who);
+    return few_rows(X) ? launch_few(X, W, K, sink, st, who) : launch_many(X, W, K, sink, st, who);
   };
   return dtype == CODA_F32 ? run(float{}) : dtype == CODA_BF16 ? run(bf16_t{}) : run(f16_t{});
 }

@@ -190,8 +190,9 @@ int coda_project_workspace_bytes(const coda_proj_desc* d, size_t* bytes);
  * Rows in 8 bits: int8 codes in [-127, 127], one float scale a row, the
  * value of a code being code * scale.  A row's codes lie at a 16-byte
  * address and are followed by zeros up to a multiple of 128 bytes (row
- * strides c_sm, x_sm, w_sm in bytes; of a product's operands at most 2^24).  No counterpart in the reference,
- * whose projections are float linears (src/coda_gqa_l/attention.py:396-410).
+ * strides c_sm, x_sm, w_sm in bytes; of a product's operands at most 2^24).
+ * No counterpart in the reference, whose projections are float linears
+ * (src/coda_gqa_l/attention.py:396-410).
  * dtype: CODA_F32, CODA_BF16 or CODA_F16; row strides of x, residual, out in
  * elements; rows of at most 32768 elements.
  * ---------------------------------------------------------------------- */

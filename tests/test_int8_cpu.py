@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import coda_gqa_l
-from coda_gqa_l import Int8Rows, _hip
+from coda_gqa_l import Int8Rows, _hip, linear_int8
 
 
 def test_layout_of_rows():
@@ -95,6 +95,24 @@ def test_linear_entry(change, error):
     L = _hip.lib()
     assert L.coda_linear_int8(*a.values(), None) == 1
     assert error in L.coda_last_error().decode()
+
+
+@pytest.mark.parametrize("change", [dict(M=(1 << 30) + 1), dict(n_feat=(1 << 30) + 1, o_sm=1 << 31)])
+def test_too_many_rows_of_a_product(change):
+    a = dict(dtype=1, x=P, x_sm=128, x_scales=P, M=3, D=128, w=P, w_sm=128, w_scales=P, n_feat=10, K=128, bias=None, out=P,
+             o_sm=10)
+    a.update(change)
+    L = _hip.lib()
+    assert L.coda_linear_int8(*a.values(), None) == 2
+    assert "2^30" in L.coda_last_error().decode()
+
+
+def test_more_rows_than_32_bits_count():
+    n = 1 << 31
+    r = Int8Rows(torch.zeros(1, 128, dtype=torch.int8).expand(n, 128), torch.zeros(1).expand(n), 100, torch.float32)
+    for call in (r.dequantize, lambda: linear_int8(r, r), lambda: linear_int8(torch.zeros(1, 100), r)):
+        with pytest.raises(RuntimeError, match="2147483648 rows"):
+            call()
 
 
 @pytest.mark.parametrize("change,error", [

@@ -172,6 +172,21 @@ def test_sum_in_place():
         assert torch.equal(ops[over], total) and torch.equal(codes, want.codes) and torch.equal(scales, want.scales)
 
 
+@pytest.mark.parametrize("D", [9, 600])
+def test_more_rows_than_a_launch(D):
+    """Rows past 2^21, which a second launch takes, are the rows that they
+    repeat."""
+    g, M = _gen(D), (1 << 21) + 1405
+    base, w = _rand(g, 1000, D, dtype=torch.bfloat16), _rand(g, D, dtype=torch.bfloat16)
+    at = torch.arange(M, device=DEV) % 1000
+    x = base[at]
+    r, want = quantize_rows(x), quantize_rows(base)
+    assert torch.equal(r.codes, want.codes[at]) and torch.equal(r.scales, want.scales[at])
+    assert torch.equal(r.dequantize(), want.dequantize()[at])
+    (r, total), (want, t0) = (rms_norm_int8(t, w, residual=t) for t in (x, base))
+    assert torch.equal(r.codes, want.codes[at]) and torch.equal(r.scales, want.scales[at]) and torch.equal(total, t0[at])
+
+
 # ---------------------------------------------------------------- product
 def _int8(g, rows, K):
     """Plain codes of the whole range, and scales."""
@@ -253,6 +268,17 @@ def test_a_row_is_its_own(M):
     run = lambda n: linear_int8(Int8Rows(a[:n], sa[:n], K, torch.bfloat16), w)  # noqa: E731
     y, whole = run(M), run(3000)
     assert torch.equal(y, whole[:M]) and torch.equal(run(M), y)
+
+
+@pytest.mark.parametrize("M,K,N", [(33000, 130944, 64), (600000, 100, 4096)])
+def test_offsets_past_32_bits(M, K, N):
+    """4.3 GB of codes; 2.5 G values: the rows that they repeat."""
+    g = _gen(M)
+    rows = Int8Rows.from_codes(*_int8(g, 1000, K), torch.bfloat16)
+    w = Int8Rows.from_codes(*_int8(g, N, K), torch.bfloat16)
+    many = Int8Rows(rows.codes.repeat(M // 1000, 1), rows.scales.repeat(M // 1000), K, torch.bfloat16)
+    y, want = linear_int8(many, w), linear_int8(rows, w)
+    assert all(torch.equal(part, want) for part in y.view(-1, 1000, N))
 
 
 @pytest.mark.parametrize("M", [3, 90, 1100])
