@@ -556,7 +556,7 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // to 1.6 GHz under it: 16384 x 8192 x 8192 880-900 us = 2440-2500 TOP/s, 32768
 // x 4096 x 6177 767 us; the smaller ones by what L2 and LDS deliver beside few
 // products: 1999 x 4096 x 4096 41 us, 128 x 8192 x 8192 26.
-template <int SF, int SM, int ST, typename T>
+template <int SF, int SM, int ST, int KS, typename T>
 struct TileLds {
   static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
   static constexpr int kStage = kRows * 128;    // bytes
@@ -566,17 +566,21 @@ struct TileLds {
   static constexpr int kRow = kFeats * sizeof(T) + 16;
   static constexpr int kScales = 64 * (2 * SF + SM) * sizeof(float);  // features' scales, biases, tokens' scales
   static constexpr int kOut = kWalk ? ST * kStage : 0;         // (smaller tiles: over the stages)
-  static constexpr size_t kEnd = kOut + kScales + 4 * 32 * kRow;
-  static constexpr size_t kBytes = kEnd > ST * kStage ? kEnd : ST * kStage;
+  static constexpr size_t kSums = kOut + kScales + 4 * 32 * kRow;  // of the second half of K
+  static constexpr size_t kEnd = kSums + (KS - 1) * SF * SM * 16 * 256 * sizeof(int32_t);
+  static constexpr size_t kBytes = kEnd > KS * ST * kStage ? kEnd : KS * ST * kStage;
 };
-template <int SF, int SM, int ST, typename Sink>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1 : 2))) void int8_tile(
+template <int SF, int SM, int ST, int KS, typename Sink>
+__global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1 : 2))) void int8_tile(
     const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
   typedef typename Sink::Out T;
-  typedef TileLds<SF, SM, ST, T> L;
+  typedef TileLds<SF, SM, ST, KS, T> L;
+  static_assert(KS == 1 || SF == 1, "tiles of more products a step are not split");
   extern __shared__ __attribute__((aligned(128))) char smem[];
   constexpr int BF = 64 * SF, BM = 64 * SM, NO = SF + SM, NL = 2 * NO;  // NO operands a quarter, NL loads a thread and step
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = wave & 3, part_k = KS == 1 ? 0 : wave >> 2;  // the share of K
+  char* const stages = smem + part_k * (ST * L::kStage);
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
   // in groups of 4 token tiles, so that what it has at a time shares rows in
   // its L2; its workgroups take them in turn.
@@ -603,16 +607,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
       src[i] = 16 * piece + (i < 2 * SF ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
                                         : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
     }
-    wsrc = W.p + a.f * W.sm;
-    xsrc = X.p + a.m * X.sm;
+    wsrc = W.p + a.f * W.sm + part_k * (K / KS);
+    xsrc = X.p + a.m * X.sm + part_k * (K / KS);
   };
   // the loads: tile lt's step lk, the ls-th of all, to stage lat; on to the next
   // tile at its end
-  const int steps = K / 128;
+  const int steps = K / (128 * KS);
   int tile = t0 + (int)(blockIdx.x >> 3), lt = tile, lk = 0, ls = 0, lat = 0;
   auto load1 = [&](auto c) {
     constexpr int i = decltype(c)::value;
-    tile_load16((i < 2 * SF ? wsrc : xsrc) + src[i], smem + lat + wv * 1024 + i * 4096);
+    tile_load16((i < 2 * SF ? wsrc : xsrc) + src[i], stages + lat + wv * 1024 + i * 4096);
   };
   auto next_stage = [](int at) { return at + L::kStage == ST * L::kStage ? 0 : at + L::kStage; };
   auto loaded = [&]() {
@@ -629,7 +633,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   i32x16 acc[SF][SM];
   // operands of quarter h of a step: pieces 2 h + lane / 32
   const int wf = wv >> 1, wm = wv & 1, r32 = lane & 31;
-  const uint32_t at = tile_lds(smem) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
+  const uint32_t at = tile_lds(stages) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
   constexpr bool kAhead = SF == 1;  // a whole step's operands are read ahead
   i32x4 op[kAhead ? 8 : 2][NO];
   auto read = [&](auto c, i32x4 (&o)[NO], uint32_t a) {  // operand c: SF of features, SM of tokens
@@ -738,7 +742,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   for (;;) {
     const At a = place(tile);
     float scale[3] = {0.f, 0.f, 0.f};
-    const int own = (int)threadIdx.x;
+    const int own = (int)threadIdx.x & 255;
     if (own < BF) {
       const int f = min(a.f + own, W.rows - 1);
       scale[0] = W.scales[f];
@@ -772,9 +776,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
       fs[BF + own] = scale[1];
     }
     if (own < BM) fs[2 * BF + own] = scale[2];
+    i32x4* sums = reinterpret_cast<i32x4*>(smem + L::kSums) + own;
+    if (KS == 2 && part_k)
+      each<SF * SM * 4>([&](auto c) {
+        constexpr int i = decltype(c)::value / 4, r = decltype(c)::value % 4;
+        const i32x16& s = acc[i / SM][i % SM];
+        sums[256 * decltype(c)::value] = i32x4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
+      });
     // (the loads too: the writes below do not stand before them)
     __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
+    if constexpr (KS == 2) {
+      if (part_k) return;
+      each<SF * SM * 4>([&](auto c) {
+        constexpr int i = decltype(c)::value / 4, r = decltype(c)::value % 4;
+        const i32x4 s = sums[256 * decltype(c)::value];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i / SM][i % SM][4 * r + e] += s[e];
+      });
+    }
     constexpr int N = Sink::kRun, PR = L::kFeats / N, NF = L::kFeats / 32;  // runs of a row, blocks of 32 features
     char* mine = smem + L::kOut + L::kScales + wv * 32 * L::kRow;
     const int fw = 32 * SF * wf, mw = 32 * SM * wm, fq = le % PR * N;
@@ -814,17 +834,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SF == 4 ? 1
   }
 }
 
-template <int SF, int SM, int ST, typename Sink>
+template <int SF, int SM, int ST, int KS, typename Sink>
 static int launch_tile(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  typedef TileLds<SF, SM, ST, typename Sink::Out> L;
+  typedef TileLds<SF, SM, ST, KS, typename Sink::Out> L;
   const int64_t ntf = ((int64_t)W.rows + 64 * SF - 1) / (64 * SF), ntm = ((int64_t)X.rows + 64 * SM - 1) / (64 * SM);
   const int64_t n = ntf * ntm;
   // (a grid has less than 2^32 threads; a walk's tiles are counted in 32 bits)
   if (n >= (L::kWalk ? INT_MAX / 8 : 1 << 24)) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)n);
-  const int rc = lds_limit<int8_tile<SF, SM, ST, Sink>>(L::kBytes, who);
+  const int rc = lds_limit<int8_tile<SF, SM, ST, KS, Sink>>(L::kBytes, who);
   if (rc) return rc;
   const int64_t grid = L::kWalk && n > device_cus() ? device_cus() : n;
-  hipLaunchKernelGGL((int8_tile<SF, SM, ST, Sink>), dim3((unsigned)grid), dim3(256), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
+  hipLaunchKernelGGL((int8_tile<SF, SM, ST, KS, Sink>), dim3((unsigned)grid), dim3(256 * KS), L::kBytes, st, X, W, K, (int)ntf, (int)ntm,
                      sink);
   return check_launch("int8_tile");
 }
@@ -985,11 +1005,14 @@ static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   const int64_t t44 = 56 * rounds(256, 256), t42 = 39 * rounds(256, 128), t22 = 23 * rounds(128, 128);
   const int64_t t12 = 17 * rounds(64, 128), t11 = n1 <= cus ? 15 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
   const int64_t least = std::min({t44, t42, t22, t12, t11});
-  if (t44 == least) return launch_tile<4, 4, 2>(X, W, K, sink, st, who);
-  if (t42 == least) return launch_tile<4, 2, 3>(X, W, K, sink, st, who);
-  if (t22 == least) return launch_tile<2, 2, 4>(X, W, K, sink, st, who);
-  if (t12 == least) return launch_tile<1, 2, 4>(X, W, K, sink, st, who);
-  return launch_tile<1, 1, 4>(X, W, K, sink, st, who);
+  if (t44 == least) return launch_tile<4, 4, 2, 1>(X, W, K, sink, st, who);
+  if (t42 == least) return launch_tile<4, 2, 3, 1>(X, W, K, sink, st, who);
+  if (t22 == least) return launch_tile<2, 2, 4, 1>(X, W, K, sink, st, who);
+  const bool halves = K % 256 == 0;
+  if (t12 == least)
+    return halves && tiles_of(X, W, 64, 128) <= cus ? launch_tile<1, 2, 3, 2>(X, W, K, sink, st, who)
+                                                    : launch_tile<1, 2, 4, 1>(X, W, K, sink, st, who);
+  return halves && n1 <= cus ? launch_tile<1, 1, 4, 2>(X, W, K, sink, st, who) : launch_tile<1, 1, 4, 1>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {
