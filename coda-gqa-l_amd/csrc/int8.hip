@@ -536,6 +536,65 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
   return v;
 }
 
+struct TileAt {
+  int f, m;
+};
+// Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own, t0
+// .. end, in groups of 4 token tiles, so that what it has at a time shares rows
+// in its L2; its workgroups take them in turn.
+struct TileOrder {
+  int ntf, ntm, t0, end;
+  __device__ __forceinline__ TileOrder(int ntf_, int ntm_) : ntf(ntf_), ntm(ntm_) {
+    const int n = ntf * ntm, xcd = blockIdx.x & 7, base = n >> 3, rem = n & 7;
+    t0 = xcd * base + min(xcd, rem);
+    end = t0 + base + (xcd < rem ? 1 : 0);
+  }
+  template <int BF, int BM>
+  __device__ __forceinline__ TileAt at(int t) const {
+    const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
+    return TileAt{in / gm * BF, (4 * group + in % gm) * BM};
+  }
+};
+
+// A wave's values out: through LDS (at mine, rows of ROW bytes, its own) from
+// four features of 32 tokens a lane to runs of a token's features, FEATS of
+// them at a time.  sw, sb, sx: in LDS, of its first feature and token (f0, m0).
+template <int SF, int SM, int FEATS, int ROW, typename Sink>
+__device__ __forceinline__ void tile_out(const i32x16 (&acc)[SF][SM], char* mine, const float* sw, const float* sb,
+                                         const float* sx, int le, int f0, int m0, int n_feat, int rows, const Sink& sink) {
+  typedef typename Sink::Out T;
+  constexpr int N = Sink::kRun, PR = FEATS / N, NF = FEATS / 32;  // runs of a row, blocks of 32 features
+  const int fq = le % PR * N, four = 4 * (le >> 5);
+  each<SM>([&](auto jc) {
+    constexpr int j = decltype(jc)::value;
+    const float x = sx[32 * j + (le & 31)];
+    each<SF / NF>([&](auto pc) {
+      constexpr int part = decltype(pc)::value;
+      each<4 * NF>([&](auto gc) {
+        constexpr int q = decltype(gc)::value, i = part * NF + q / 4, r = q % 4, f = 32 * i + 8 * r;
+        const pf32x4 w = *reinterpret_cast<const pf32x4*>(sw + four + f), b = *reinterpret_cast<const pf32x4*>(sb + four + f);
+        i32x4 v;
+        each<4>([&](auto ec) {
+          constexpr int e = decltype(ec)::value;
+          v[e] = SF == 4 ? acc_read(acc[i][j][4 * r + e]) : acc[i][j][4 * r + e];
+        });
+        *reinterpret_cast<Feats<T, 4>*>(mine + (le & 31) * ROW + (32 * (q / 4) + 8 * r + four) * sizeof(T)) =
+            int8_value<T>(v, x, w, b);
+      });
+      __builtin_amdgcn_wave_barrier();
+      const int f = f0 + part * FEATS + fq;
+      const typename Sink::Lane to = sink.lane(min(f, n_feat - 1));
+      constexpr int R = PR / 2;  // of 32 tokens: 64 / PR a turn
+      Feats<T, N> v[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        v[r] = *reinterpret_cast<const Feats<T, N>*>(mine + (r * (64 / PR) + le / PR) * ROW + fq * sizeof(T));
+      if (f < n_feat) sink.put(to, m0 + 32 * j + le / PR, 64 / PR, rows, v);
+      __builtin_amdgcn_wave_barrier();
+    });
+  });
+}
+
 // 4 waves (2 x 2) make 64 SF features x 64 SM tokens, a wave 32 SF x 32 SM in
 // SF x SM accumulators of 32 x 32.  K passes through LDS in steps of 128 bytes
 // (whole lines: rows of 64 bytes come out of L2 at 70 GB/s a CU, of 128 at
@@ -549,13 +608,15 @@ __device__ __forceinline__ int32_t acc_read(int32_t a) {
 // the barrier is at a step's start.  A stage holds a row's eight 16-byte pieces in the
 // order slot = piece ^ (row / 2) % 8, by which the 16 lanes that LDS serves at
 // once (of 32 rows: 0-3, 12-15, 20-27 and the rest) touch every bank once.
+// KS = 2: two sets of four waves, a half of K and a ring of stages each; the
+// second set's sums pass through LDS at the end.
 // A workgroup of the largest tiles goes from tile to tile; the stages run on
 // over the border, so that the next tile's first steps are in LDS when this
 // one's values have been written, and the writes are on their way while its
 // products run.  Those are bound by the matrix pipe, whose clock falls to 1.25
 // to 1.6 GHz under it: 16384 x 8192 x 8192 880-900 us = 2440-2500 TOP/s, 32768
 // x 4096 x 6177 767 us; the smaller ones by what L2 and LDS deliver beside few
-// products: 1999 x 4096 x 4096 41 us, 128 x 8192 x 8192 26.
+// products: 1999 x 4096 x 4096 41 us, 128 x 8192 x 10305 33.
 template <int SF, int SM, int ST, int KS, typename T>
 struct TileLds {
   static constexpr int kRows = 64 * (SF + SM);  // features, then tokens
@@ -581,24 +642,14 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = wave & 3, part_k = KS == 1 ? 0 : wave >> 2;  // the share of K
   char* const stages = smem + part_k * (ST * L::kStage);
-  // Workgroups go round the 8 XCDs; each XCD takes a run of tiles of its own,
-  // in groups of 4 token tiles, so that what it has at a time shares rows in
-  // its L2; its workgroups take them in turn.
-  const int n = ntf * ntm, xcd = blockIdx.x & 7, base = n >> 3, rem = n & 7;
-  const int t0 = xcd * base + min(xcd, rem), end = t0 + base + (xcd < rem ? 1 : 0);
-  const int turn = ((int)gridDim.x - xcd + 7) >> 3;
-  struct At {
-    int f, m;
-  };
-  auto place = [&](int t) {
-    const int group = t / (4 * ntf), in = t - group * 4 * ntf, gm = min(4, ntm - 4 * group);
-    return At{in / gm * BF, (4 * group + in % gm) * BM};
-  };
+  const TileOrder order(ntf, ntm);
+  const int t0 = order.t0, end = order.end, turn = ((int)gridDim.x - (int)(blockIdx.x & 7) + 7) >> 3;
+  const auto place = [&](int t) { return order.at<BF, BM>(t); };
   // this lane's pieces, as offsets from a tile's first rows: a load is 8 rows
   // of eight pieces, the first 2 SF of them features
   uint32_t src[NL];
   const int8_t *wsrc, *xsrc;
-  auto aim = [&](const At& a) {
+  auto aim = [&](const TileAt& a) {
     int l = lane;
     asm volatile("" : "+v"(l));  // (nothing of this is worth a register between tiles)
 #pragma unroll
@@ -740,7 +791,7 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 
     tile_landed(op[h]);
   });
   for (;;) {
-    const At a = place(tile);
+    const TileAt a = place(tile);
     float scale[3] = {0.f, 0.f, 0.f};
     const int own = (int)threadIdx.x & 255;
     if (own < BF) {
@@ -765,8 +816,6 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 
     } else {
       for (int k = 0; k < steps; ++k) step();
     }
-    // Values pass through LDS (a wave's own part) from four features of 32
-    // tokens a lane to runs of a token's features
     int le = lane;
     asm volatile("" : "+v"(le));  // (nor are these addresses)
     if (!L::kWalk) __builtin_amdgcn_s_barrier();  // every wave has read its last operands
@@ -795,43 +844,156 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 
         for (int e = 0; e < 4; ++e) acc[i / SM][i % SM][4 * r + e] += s[e];
       });
     }
-    constexpr int N = Sink::kRun, PR = L::kFeats / N, NF = L::kFeats / 32;  // runs of a row, blocks of 32 features
-    char* mine = smem + L::kOut + L::kScales + wv * 32 * L::kRow;
-    const int fw = 32 * SF * wf, mw = 32 * SM * wm, fq = le % PR * N;
-    const float* fl = fs + fw + 4 * (le >> 5);
-    each<SM>([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      const float sx = fs[2 * BF + mw + 32 * j + (le & 31)];
-      each<SF / NF>([&](auto pc) {
-        constexpr int part = decltype(pc)::value;
-        each<4 * NF>([&](auto gc) {
-          constexpr int q = decltype(gc)::value, i = part * NF + q / 4, r = q % 4, f = 32 * i + 8 * r;
-          const pf32x4 sw = *reinterpret_cast<const pf32x4*>(fl + f);
-          const pf32x4 bias = *reinterpret_cast<const pf32x4*>(fl + BF + f);
-          i32x4 v;
-          each<4>([&](auto ec) {
-            constexpr int e = decltype(ec)::value;
-            v[e] = SF == 4 ? acc_read(acc[i][j][4 * r + e]) : acc[i][j][4 * r + e];
-          });
-          *reinterpret_cast<Feats<T, 4>*>(mine + (le & 31) * L::kRow + (32 * (q / 4) + 8 * r + 4 * (le >> 5)) * sizeof(T)) =
-              int8_value<T>(v, sx, sw, bias);
-        });
-        __builtin_amdgcn_wave_barrier();
-        const int f = a.f + fw + part * L::kFeats + fq;
-        const typename Sink::Lane to = sink.lane(min(f, W.rows - 1));
-        constexpr int R = PR / 2;  // of 32 tokens: 64 / PR a turn
-        Feats<T, N> v[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          v[r] = *reinterpret_cast<const Feats<T, N>*>(mine + (r * (64 / PR) + le / PR) * L::kRow + fq * sizeof(T));
-        if (f < W.rows) sink.put(to, a.m + mw + 32 * j + le / PR, 64 / PR, X.rows, v);
-        __builtin_amdgcn_wave_barrier();
-      });
-    });
+    const int fw = 32 * SF * wf, mw = 32 * SM * wm;
+    tile_out<SF, SM, L::kFeats, L::kRow>(acc, smem + L::kOut + L::kScales + wv * 32 * L::kRow, fs + fw, fs + BF + fw,
+                                         fs + 2 * BF + mw, le, a.f + fw, a.m + mw, W.rows, X.rows, sink);
     if (!L::kWalk) break;
     tile += turn;
     if (tile >= end) break;
   }
+}
+
+// A tile of 64 x 64 of whose K each of 4 waves takes a quarter, in steps of 128
+// bytes through two LDS stages of its own: no wave waits for another, and every
+// operand passes LDS once (in int8_tile twice).  Beside the first half of a
+// step's 16 products the step after next is asked for, into the stage whose
+// operands are in registers by now; beside the second half the next step's
+// operands are read.  Then the waves exchange sums, each to a block of 32 x 32.
+// Bound by a CU's loads (a MiB in 14 us at 128 x 8192 x 4096).  us, weights in
+// cache | not, beside int8_tile<1, 1, 4, 1>: 128 x 8192 x 8192 17.4 | 22.7 and
+// 25.5 | 26.1, 128 x 8192 x 4096 15.2 | 20.1 and 24.1 | 23.1, 256 x 4096 x 4096
+// 10.6 | 11.4 and 14.8 | 13.5, 200 x 512 x 1024 4.2 both.  With two sets of four
+// waves and halves of K 24.0, 21.6 and 12.4 (weights not in cache), with eight
+// waves of a stage each 24.0, 21.1 and 11.8.
+template <typename Sink>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void int8_quarters(
+    const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
+  typedef typename Sink::Out T;
+  extern __shared__ __attribute__((aligned(128))) char smem[];
+  constexpr int NL = 16, kStage = 128 * 128;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const TileOrder order(ntf, ntm);
+  const TileAt a = order.at<64, 64>(order.t0 + (int)(blockIdx.x >> 3));
+  char* const mine = smem + wv * (2 * kStage);
+  const int steps = K / 128, first = steps * wv / 4, np = steps * (wv + 1) / 4 - first;
+  uint32_t src[NL];  // a load: 8 rows of eight pieces (their order in LDS as in int8_tile)
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int r = 8 * (i & 7) + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+    src[i] = 16 * piece + (i < 8 ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
+                                 : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
+  }
+  const int8_t *wsrc = W.p + a.f * W.sm + first * 128, *xsrc = X.p + a.m * X.sm + first * 128;
+  auto load1 = [&](auto c, int stage) {
+    constexpr int i = decltype(c)::value;
+    tile_load16((i < 8 ? wsrc : xsrc) + src[i], mine + stage * kStage + i * 1024);
+  };
+  auto loaded = [&]() {
+    wsrc += 128;
+    xsrc += 128;
+  };
+  // operands of quarter h of a step: pieces 2 h + lane / 32; two of features,
+  // two of tokens
+  const int r32 = lane & 31;
+  const uint32_t at = tile_lds(mine) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
+  i32x4 op[8][4];
+  i32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i / 2][i % 2][e] = 0;
+  auto read = [&](auto c, auto set) {  // operand c of 16, of the step in stage set
+    constexpr int h = decltype(c)::value / 4, i = decltype(c)::value % 4, st = decltype(set)::value;
+    op[4 * st + h][i] = tile_read<st * kStage + i * 4096>(at ^ (32 * h));
+  };
+  auto step = [&](auto set, int behind) {  // behind: steps left after this one
+    constexpr int now = decltype(set)::value, next = 1 - now;
+    const bool ask = behind >= 2;
+    each<16>([&](auto c) {
+      constexpr int p = decltype(c)::value, h = p / 4, i = p % 4 / 2, j = p % 2;
+      if constexpr (p < 8)
+        if (ask) {
+          load1(std::integral_constant<int, 2 * p>{}, now);
+          load1(std::integral_constant<int, 2 * p + 1>{}, now);
+        }
+      if constexpr (p == 8) {  // the next step has landed
+        if (ask) __builtin_amdgcn_s_waitcnt((NL & 15) | (NL >> 4) << 14 | 0x0f70);
+        else __builtin_amdgcn_s_waitcnt(0x0f70);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (p >= 8) {
+        read(std::integral_constant<int, 2 * p - 16>{}, std::integral_constant<int, next>{});
+        read(std::integral_constant<int, 2 * p - 15>{}, std::integral_constant<int, next>{});
+      }
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[4 * now + h][i], op[4 * now + h][2 + j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    each<4>([&](auto h) { tile_landed(op[4 * next + decltype(h)::value]); });
+    if (ask) loaded();
+  };
+  float* fs = reinterpret_cast<float*>(smem + kStage + 8192);  // scales and biases of features, scales of tokens
+  float scale[3] = {0.f, 0.f, 0.f};
+  const int own = (int)threadIdx.x;
+  if (own < 64) {
+    const int f = min(a.f + own, W.rows - 1);
+    scale[0] = W.scales[f];
+    scale[1] = sink.bias1(f);
+    scale[2] = X.scales[min(a.m + own, X.rows - 1)];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  for (int s = 0; s < 2 && s < np; ++s) {
+    each<NL>([&](auto c) { load1(c, s); });
+    loaded();
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (np > 1) __builtin_amdgcn_s_waitcnt((NL & 15) | (NL >> 4) << 14 | 0x0f70);
+  else __builtin_amdgcn_s_waitcnt(0x0f70);
+  __builtin_amdgcn_sched_barrier(0);
+  each<16>([&](auto c) { read(c, std::integral_constant<int, 0>{}); });
+  each<4>([&](auto h) { tile_landed(op[decltype(h)::value]); });
+  int k = 0;
+  for (; k + 1 < np; k += 2) {
+    step(std::integral_constant<int, 0>{}, np - 1 - k);
+    step(std::integral_constant<int, 1>{}, np - 2 - k);
+  }
+  if (k < np) step(std::integral_constant<int, 0>{}, 0);
+  // A wave's sums over its first stage, the values and the scales over second ones
+  i32x4* sums = reinterpret_cast<i32x4*>(smem) + lane;
+  constexpr int kWave = 2 * kStage / 16;  // from wave to wave
+  each<16>([&](auto c) {
+    constexpr int b = decltype(c)::value / 4, r = decltype(c)::value % 4;
+    const i32x16& s = acc[b / 2][b % 2];
+    sums[wv * kWave + 64 * decltype(c)::value] = i32x4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
+  });
+  if (own < 64) {
+    fs[own] = scale[0];
+    fs[64 + own] = scale[1];
+    fs[128 + own] = scale[2];
+  }
+  __syncthreads();
+  i32x16 total[1][1];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    i32x4 t = sums[64 * (4 * wv + r)];
+#pragma unroll
+    for (int o = 1; o < 4; ++o) t += sums[o * kWave + 64 * (4 * wv + r)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) total[0][0][4 * r + e] = t[e];
+  }
+  const int fw = 32 * (wv >> 1), mw = 32 * (wv & 1);
+  tile_out<1, 1, 32, 32 * sizeof(T) + 16>(total, mine + kStage, fs + fw, fs + 64 + fw, fs + 128 + mw, lane, a.f + fw,
+                                          a.m + mw, W.rows, X.rows, sink);
+}
+
+template <typename Sink>
+static int launch_quarters(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
+  constexpr size_t kBytes = 4 * 2 * 128 * 128;
+  const int ntf = (W.rows + 63) / 64, ntm = (X.rows + 63) / 64;
+  if ((int64_t)ntf * ntm >= 1 << 24) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)ntf * ntm);
+  const int rc = lds_limit<int8_quarters<Sink>>(kBytes, who);
+  if (rc) return rc;
+  hipLaunchKernelGGL((int8_quarters<Sink>), dim3(ntf * ntm), dim3(256), kBytes, st, X, W, K, ntf, ntm, sink);
+  return check_launch("int8_quarters");
 }
 
 template <int SF, int SM, int ST, int KS, typename Sink>
@@ -989,30 +1151,33 @@ static int64_t tiles_of(const Int8Mat& X, const Int8Mat& W, int f, int m) {
 // The row kernels or tiles: up to 64 rows the former (us, rows and tiles: 17 x
 // 4096 x 6177 11.5 and 14.2, 64 x 4096 x 4096 10.0 and 12.9, 64 x 8192 x 8192
 // 24.7 and 26.8, 64 x 4096 x 6177 14.6 and 13.7, 128 x 4096 x 6177 19.2 and
-// 13.7, 128 x 8192 x 8192 32.0 and 26.4, 128 x 8192 x 10305 38.1 and 33.0).
+// 13.7, 128 x 8192 x 8192 32.0 and 22.7, 128 x 8192 x 10305 38.1 and 33.1).
 static bool few_rows(const Int8Mat& X) { return X.rows <= 64; }
 // The tile by the time that its rounds take, us a round of one tile (64 x 64:
 // two) a CU at K = 4096.  Measured, 256 x 256 | 256 x 128 | 128 x 128 | 64 x
 // 128 | 64 x 64 (features x tokens): 1999 x 4096 x 4096 55 41 50 - 75, 1999 x
 // 4096 x 6177 58 68 81 - 107, 1000 x 4096 x 4096 52 31 24 35 38, 300 x 4096 x
 // 6177 - 37 20 32 21, 500 x 2048 x 3105 - 19 12.5 10.6 10.8, 128 x 8192 x
-// 10305 - - 43 33 41, 128 x 8192 x 8192 - - 42 32 26, 4096 x 4096 x 6177 112
+// 10305 - - 43 33 41, 128 x 8192 x 8192 - - 42 31 23, 4096 x 4096 x 6177 112
 // 130 157 - -, 2000 x 1024 x 1024 - - 9.3 - 8.1.
 template <typename Sink>
 static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
   const int64_t cus = device_cus(), n1 = tiles_of(X, W, 64, 64);
   const auto rounds = [&](int f, int m) { return (tiles_of(X, W, f, m) + cus - 1) / cus; };
   const int64_t t44 = 56 * rounds(256, 256), t42 = 39 * rounds(256, 128), t22 = 23 * rounds(128, 128);
-  const int64_t t12 = 17 * rounds(64, 128), t11 = n1 <= cus ? 15 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
+  const int64_t t12 = 17 * rounds(64, 128), t11 = n1 <= cus ? 12 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
   const int64_t least = std::min({t44, t42, t22, t12, t11});
   if (t44 == least) return launch_tile<4, 4, 2, 1>(X, W, K, sink, st, who);
   if (t42 == least) return launch_tile<4, 2, 3, 1>(X, W, K, sink, st, who);
   if (t22 == least) return launch_tile<2, 2, 4, 1>(X, W, K, sink, st, who);
+  // (64 x 128 in one round: a workgroup a CU anyway, so with a second set of
+  // waves for half of K, if it has halves of whole steps: 250 x 4096 x 6177 18.6
+  // -> 17.0, 128 x 8192 x 10305 33.6 -> 33.1)
   const bool halves = K % 256 == 0;
   if (t12 == least)
     return halves && tiles_of(X, W, 64, 128) <= cus ? launch_tile<1, 2, 3, 2>(X, W, K, sink, st, who)
                                                     : launch_tile<1, 2, 4, 1>(X, W, K, sink, st, who);
-  return halves && n1 <= cus ? launch_tile<1, 1, 4, 2>(X, W, K, sink, st, who) : launch_tile<1, 1, 4, 1>(X, W, K, sink, st, who);
+  return n1 <= cus ? launch_quarters(X, W, K, sink, st, who) : launch_tile<1, 1, 4, 1>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {

@@ -219,6 +219,18 @@ def test_linear_int8(M, K, N, dtype):
     _check_product(linear_int8(x, w, bias), a, sa, b, sb, bias)
 
 
+@pytest.mark.parametrize("K", [1, 128, 129, 300, 384, 512, 520, 640, 896, 1000, 1152])
+@pytest.mark.parametrize("M,N", [(70, 500), (200, 1030), (128, 10305), (130, 9000), (250, 4100)])
+def test_shares_of_k(M, K, N):
+    """Few and odd numbers of steps where several waves share K: some have one
+    step more than others, or none."""
+    g = _gen(K + M)
+    (a, sa), (b, sb) = _int8(g, M, K), _int8(g, N, K)
+    bias = _rand(g, N, dtype=torch.bfloat16)
+    y = linear_int8(Int8Rows.from_codes(a, sa, torch.bfloat16), Int8Rows.from_codes(b, sb, torch.bfloat16), bias)
+    _check_product(y, a, sa, b, sb, bias)
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_longest_sum(M):
     """Codes of 127 all along the longest row: just below 2^31."""
