@@ -511,6 +511,8 @@ __device__ __forceinline__ void tile_landed(i32x4 (&a)[N]) {
   if constexpr (N == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]));
   if constexpr (N == 3) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]));
   if constexpr (N == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+  if constexpr (N == 5)
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]));
   if constexpr (N == 6)
     asm volatile("s_waitcnt lgkmcnt(0)"
                  : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]));
@@ -853,93 +855,97 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(SF == 
   }
 }
 
-// A tile of 64 x 64 of whose K each of 4 waves takes a quarter, in steps of 128
+// A tile of 32 FB features x 64 tokens of whose K each of 4 waves takes a quarter, in steps of 128
 // bytes through two LDS stages of its own: no wave waits for another, and every
 // operand passes LDS once (in int8_tile twice).  Beside the first half of a
-// step's 16 products the step after next is asked for, into the stage whose
+// step's 8 FB products the step after next is asked for, into the stage whose
 // operands are in registers by now; beside the second half the next step's
-// operands are read.  Then the waves exchange sums, each to a block of 32 x 32.
+// operands are read.  Then the waves exchange sums and write blocks of 32 x 32.
 // Bound by a CU's loads (a MiB in 14 us at 128 x 8192 x 4096).  us, weights in
 // cache | not, beside int8_tile<1, 1, 4, 1>: 128 x 8192 x 8192 17.4 | 22.7 and
 // 25.5 | 26.1, 128 x 8192 x 4096 15.2 | 20.1 and 24.1 | 23.1, 256 x 4096 x 4096
 // 10.6 | 11.4 and 14.8 | 13.5, 200 x 512 x 1024 4.2 both.  With two sets of four
 // waves and halves of K 24.0, 21.6 and 12.4 (weights not in cache), with eight
 // waves of a stage each 24.0, 21.1 and 11.8.
-template <typename Sink>
+template <int FB, typename Sink>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void int8_quarters(
     const Int8Mat X, const Int8Mat W, int K, int ntf, int ntm, const Sink sink) {
   typedef typename Sink::Out T;
   extern __shared__ __attribute__((aligned(128))) char smem[];
-  constexpr int NL = 16, kStage = 128 * 128;
+  constexpr int BF = 32 * FB, NO = FB + 2, NL = 4 * NO, NP = 8 * FB, kStage = (BF + 64) * 128;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const TileOrder order(ntf, ntm);
-  const TileAt a = order.at<64, 64>(order.t0 + (int)(blockIdx.x >> 3));
+  const TileAt a = order.at<BF, 64>(order.t0 + (int)(blockIdx.x >> 3));
+  // of a ring: a wave's sums, then (at kOut) its values
+  constexpr int kSums = FB * 2 * 4096, kRow = 32 * sizeof(T) + 16, kOut = kSums + 4 * (2 * BF + 64);
+  static_assert(kOut + 32 * kRow <= 2 * kStage, "the exchange lies in the rings");
   char* const mine = smem + wv * (2 * kStage);
   const int steps = K / 128, first = steps * wv / 4, np = steps * (wv + 1) / 4 - first;
   uint32_t src[NL];  // a load: 8 rows of eight pieces (their order in LDS as in int8_tile)
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int r = 8 * (i & 7) + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
-    src[i] = 16 * piece + (i < 8 ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
+    const int r = 8 * (i < 4 * FB ? i : i - 4 * FB) + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+    src[i] = 16 * piece + (i < 4 * FB ? (uint32_t)min(r, W.rows - 1 - a.f) * (uint32_t)W.sm
                                  : (uint32_t)min(r, X.rows - 1 - a.m) * (uint32_t)X.sm);
   }
   const int8_t *wsrc = W.p + a.f * W.sm + first * 128, *xsrc = X.p + a.m * X.sm + first * 128;
   auto load1 = [&](auto c, int stage) {
     constexpr int i = decltype(c)::value;
-    tile_load16((i < 8 ? wsrc : xsrc) + src[i], mine + stage * kStage + i * 1024);
+    tile_load16((i < 4 * FB ? wsrc : xsrc) + src[i], mine + stage * kStage + i * 1024);
   };
   auto loaded = [&]() {
     wsrc += 128;
     xsrc += 128;
   };
-  // operands of quarter h of a step: pieces 2 h + lane / 32; two of features,
+  // operands of quarter h of a step: pieces 2 h + lane / 32; FB of features,
   // two of tokens
   const int r32 = lane & 31;
   const uint32_t at = tile_lds(mine) + r32 * 128 + (((lane >> 5) ^ ((r32 >> 1) & 7)) << 4);
-  i32x4 op[8][4];
-  i32x16 acc[2][2];
+  i32x4 op[8][NO];
+  i32x16 acc[FB][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2 * FB; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i / 2][i % 2][e] = 0;
-  auto read = [&](auto c, auto set) {  // operand c of 16, of the step in stage set
-    constexpr int h = decltype(c)::value / 4, i = decltype(c)::value % 4, st = decltype(set)::value;
+  auto read = [&](auto c, auto set) {  // operand c of NL, of the step in stage set
+    constexpr int h = decltype(c)::value / NO, i = decltype(c)::value % NO, st = decltype(set)::value;
     op[4 * st + h][i] = tile_read<st * kStage + i * 4096>(at ^ (32 * h));
   };
   auto step = [&](auto set, int behind) {  // behind: steps left after this one
     constexpr int now = decltype(set)::value, next = 1 - now;
     const bool ask = behind >= 2;
-    each<16>([&](auto c) {
-      constexpr int p = decltype(c)::value, h = p / 4, i = p % 4 / 2, j = p % 2;
-      if constexpr (p < 8)
+    each<NP>([&](auto c) {
+      constexpr int p = decltype(c)::value, h = p / (2 * FB), i = p % (2 * FB) / 2, j = p % 2, late = p - NP / 2;
+      if constexpr (2 * p < NL)
         if (ask) {
           load1(std::integral_constant<int, 2 * p>{}, now);
           load1(std::integral_constant<int, 2 * p + 1>{}, now);
         }
-      if constexpr (p == 8) {  // the next step has landed
+      if constexpr (late == 0) {  // the next step has landed
         if (ask) __builtin_amdgcn_s_waitcnt((NL & 15) | (NL >> 4) << 14 | 0x0f70);
         else __builtin_amdgcn_s_waitcnt(0x0f70);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (p >= 8) {
-        read(std::integral_constant<int, 2 * p - 16>{}, std::integral_constant<int, next>{});
-        read(std::integral_constant<int, 2 * p - 15>{}, std::integral_constant<int, next>{});
+      if constexpr (late >= 0 && 2 * late < NL) {
+        read(std::integral_constant<int, 2 * late>{}, std::integral_constant<int, next>{});
+        read(std::integral_constant<int, 2 * late + 1>{}, std::integral_constant<int, next>{});
       }
-      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[4 * now + h][i], op[4 * now + h][2 + j], acc[i][j], 0, 0, 0);
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[4 * now + h][i], op[4 * now + h][FB + j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
     each<4>([&](auto h) { tile_landed(op[4 * next + decltype(h)::value]); });
     if (ask) loaded();
   };
-  float* fs = reinterpret_cast<float*>(smem + kStage + 8192);  // scales and biases of features, scales of tokens
+  // (the values and the scales over the ends of rings)
+  float* fs = reinterpret_cast<float*>(smem + kOut - 4 * (2 * BF + 64));  // of features, their biases, of tokens
   float scale[3] = {0.f, 0.f, 0.f};
   const int own = (int)threadIdx.x;
-  if (own < 64) {
+  if (own < BF) {
     const int f = min(a.f + own, W.rows - 1);
     scale[0] = W.scales[f];
     scale[1] = sink.bias1(f);
-    scale[2] = X.scales[min(a.m + own, X.rows - 1)];
   }
+  if (own < 64) scale[2] = X.scales[min(a.m + own, X.rows - 1)];
   __builtin_amdgcn_sched_barrier(0);
   for (int s = 0; s < 2 && s < np; ++s) {
     each<NL>([&](auto c) { load1(c, s); });
@@ -949,7 +955,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void i
   if (np > 1) __builtin_amdgcn_s_waitcnt((NL & 15) | (NL >> 4) << 14 | 0x0f70);
   else __builtin_amdgcn_s_waitcnt(0x0f70);
   __builtin_amdgcn_sched_barrier(0);
-  each<16>([&](auto c) { read(c, std::integral_constant<int, 0>{}); });
+  each<NL>([&](auto c) { read(c, std::integral_constant<int, 0>{}); });
   each<4>([&](auto h) { tile_landed(op[decltype(h)::value]); });
   int k = 0;
   for (; k + 1 < np; k += 2) {
@@ -957,42 +963,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void i
     step(std::integral_constant<int, 1>{}, np - 2 - k);
   }
   if (k < np) step(std::integral_constant<int, 0>{}, 0);
-  // A wave's sums over its first stage, the values and the scales over second ones
   i32x4* sums = reinterpret_cast<i32x4*>(smem) + lane;
   constexpr int kWave = 2 * kStage / 16;  // from wave to wave
-  each<16>([&](auto c) {
+  each<NP>([&](auto c) {
     constexpr int b = decltype(c)::value / 4, r = decltype(c)::value % 4;
     const i32x16& s = acc[b / 2][b % 2];
     sums[wv * kWave + 64 * decltype(c)::value] = i32x4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
   });
-  if (own < 64) {
-    fs[own] = scale[0];
-    fs[64 + own] = scale[1];
-    fs[128 + own] = scale[2];
-  }
+  // (the scales lie in wave 0's ring: behind its loop only by a barrier)
   __syncthreads();
-  i32x16 total[1][1];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    i32x4 t = sums[64 * (4 * wv + r)];
-#pragma unroll
-    for (int o = 1; o < 4; ++o) t += sums[o * kWave + 64 * (4 * wv + r)];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) total[0][0][4 * r + e] = t[e];
+  if (own < BF) {
+    fs[own] = scale[0];
+    fs[BF + own] = scale[1];
   }
-  const int fw = 32 * (wv >> 1), mw = 32 * (wv & 1);
-  tile_out<1, 1, 32, 32 * sizeof(T) + 16>(total, mine + kStage, fs + fw, fs + 64 + fw, fs + 128 + mw, lane, a.f + fw,
-                                          a.m + mw, W.rows, X.rows, sink);
+  if (own < 64) fs[2 * BF + own] = scale[2];
+  __syncthreads();
+  for (int b = wv; b < 2 * FB; b += 4) {
+    i32x16 total[1][1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      i32x4 t = sums[64 * (4 * b + r)];
+#pragma unroll
+      for (int o = 1; o < 4; ++o) t += sums[o * kWave + 64 * (4 * b + r)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[0][0][4 * r + e] = t[e];
+    }
+    const int fw = 32 * (b >> 1), mw = 32 * (b & 1);
+    tile_out<1, 1, 32, kRow>(total, mine + kOut, fs + fw, fs + BF + fw, fs + 2 * BF + mw, lane, a.f + fw, a.m + mw, W.rows,
+                             X.rows, sink);
+  }
 }
 
-template <typename Sink>
+template <int FB, typename Sink>
 static int launch_quarters(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sink, hipStream_t st, const char* who) {
-  constexpr size_t kBytes = 4 * 2 * 128 * 128;
-  const int ntf = (W.rows + 63) / 64, ntm = (X.rows + 63) / 64;
+  constexpr size_t kBytes = 4 * 2 * (32 * FB + 64) * 128;
+  const int ntf = (W.rows + 32 * FB - 1) / (32 * FB), ntm = (X.rows + 63) / 64;
   if ((int64_t)ntf * ntm >= 1 << 24) return fail(CODA_EUNSUP, "%s: %lld tiles", who, (long long)ntf * ntm);
-  const int rc = lds_limit<int8_quarters<Sink>>(kBytes, who);
+  const int rc = lds_limit<int8_quarters<FB, Sink>>(kBytes, who);
   if (rc) return rc;
-  hipLaunchKernelGGL((int8_quarters<Sink>), dim3(ntf * ntm), dim3(256), kBytes, st, X, W, K, ntf, ntm, sink);
+  hipLaunchKernelGGL((int8_quarters<FB, Sink>), dim3(ntf * ntm), dim3(256), kBytes, st, X, W, K, ntf, ntm, sink);
   return check_launch("int8_quarters");
 }
 
@@ -1148,11 +1157,20 @@ static int launch_few(const Int8Mat& X, const Int8Mat& W, int K, const Sink& sin
 static int64_t tiles_of(const Int8Mat& X, const Int8Mat& W, int f, int m) {
   return ((int64_t)W.rows + f - 1) / f * (((int64_t)X.rows + m - 1) / m);
 }
-// The row kernels or tiles: up to 64 rows the former (us, rows and tiles: 17 x
-// 4096 x 6177 11.5 and 14.2, 64 x 4096 x 4096 10.0 and 12.9, 64 x 8192 x 8192
-// 24.7 and 26.8, 64 x 4096 x 6177 14.6 and 13.7, 128 x 4096 x 6177 19.2 and
-// 13.7, 128 x 8192 x 8192 32.0 and 22.7, 128 x 8192 x 10305 38.1 and 33.1).
-static bool few_rows(const Int8Mat& X) { return X.rows <= 64; }
+// The row kernels or tiles: the former up to 32 rows, and up to 64 where there
+// are few features (us, rows and tiles, weights not in cache | in cache: 32 x
+// 4096 x 4096 7.6 | 7.3 and 10.8 | 9.2, 32 x 8192 x 8192 21.5 | 19.5 and 23.7 |
+// 15.1, 64 x 4096 x 4096 9.5 | 9.0 and 12.0 | 9.2, 64 x 4096 x 6177 14.7 | 12.7
+// and 13.8 | 9.7, 64 x 8192 x 8192 24.5 | 22.0 and 25.4 | 16.4, 64 x 8192 x
+// 10305 31.8 | 26.6 and 28.3 | 18.2).
+static bool few_rows(const Int8Mat& X, const Int8Mat& W) { return X.rows <= (W.rows < 6144 ? 64 : 32); }
+// Whether tiles of 96 x 64 save a second round of 64 x 64 (weights not in cache |
+// in cache, us, the best of the others and this: 128 x 8192 x 10305 33.9 | 24.0
+// and 30.8 | 21.0, 250 x 4096 x 6000 16.9 | 15.4 and 15.8 | 13.2, 128 x 1024 x
+// 9000 7.1 | 7.8 and 7.5 | 8.0)
+static bool one_round_of_96(const Int8Mat& X, const Int8Mat& W, int K) {
+  return K >= 2048 && tiles_of(X, W, 64, 64) > device_cus() && tiles_of(X, W, 96, 64) <= device_cus();
+}
 // The tile by the time that its rounds take, us a round of one tile (64 x 64:
 // two) a CU at K = 4096.  Measured, 256 x 256 | 256 x 128 | 128 x 128 | 64 x
 // 128 | 64 x 64 (features x tokens): 1999 x 4096 x 4096 55 41 50 - 75, 1999 x
@@ -1166,7 +1184,9 @@ static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   const auto rounds = [&](int f, int m) { return (tiles_of(X, W, f, m) + cus - 1) / cus; };
   const int64_t t44 = 56 * rounds(256, 256), t42 = 39 * rounds(256, 128), t22 = 23 * rounds(128, 128);
   const int64_t t12 = 17 * rounds(64, 128), t11 = n1 <= cus ? 12 : 19 * ((n1 + 2 * cus - 1) / (2 * cus));
-  const int64_t least = std::min({t44, t42, t22, t12, t11});
+  const int64_t t31 = one_round_of_96(X, W, K) ? 15 : INT_MAX;
+  const int64_t least = std::min({t44, t42, t22, t12, t31, t11});
+  if (t31 == least) return launch_quarters<3>(X, W, K, sink, st, who);
   if (t44 == least) return launch_tile<4, 4, 2, 1>(X, W, K, sink, st, who);
   if (t42 == least) return launch_tile<4, 2, 3, 1>(X, W, K, sink, st, who);
   if (t22 == least) return launch_tile<2, 2, 4, 1>(X, W, K, sink, st, who);
@@ -1177,7 +1197,7 @@ static int launch_many(const Int8Mat& X, const Int8Mat& W, int K, const Sink& si
   if (t12 == least)
     return halves && tiles_of(X, W, 64, 128) <= cus ? launch_tile<1, 2, 3, 2>(X, W, K, sink, st, who)
                                                     : launch_tile<1, 2, 4, 1>(X, W, K, sink, st, who);
-  return n1 <= cus ? launch_quarters(X, W, K, sink, st, who) : launch_tile<1, 1, 4, 1>(X, W, K, sink, st, who);
+  return n1 <= cus ? launch_quarters<2>(X, W, K, sink, st, who) : launch_tile<1, 1, 4, 1>(X, W, K, sink, st, who);
 }
 
 static int check_codes_out(const int8_t* codes, int64_t c_sm, const float* scales, int rows, int D, const char* who) {
@@ -1276,7 +1296,7 @@ extern "C" int coda_linear_int8(int dtype, const void* x, int64_t x_sm, const fl
     typedef decltype(t) T;
     const LinearSink<T> sink{(T*)out, (const T*)bias, o_sm, n_feat};
     if (!x_scales) return launch_of<T>(x, x_sm, M, D, W, K, sink, st, who);
-    return few_rows(X) ? launch_few(X, W, K, sink, st, who) : launch_many(X, W, K, sink, st, who);
+    return few_rows(X, W) ? launch_few(X, W, K, sink, st, who) : launch_many(X, W, K, sink, st, who);
   };
   return dtype == CODA_F32 ? run(float{}) : dtype == CODA_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
@@ -1317,8 +1337,9 @@ extern "C" int coda_project_int8(const coda_proj_desc* d, const float* x_scales,
     const FrontSink<T, true, 4> few{*d, tab, len, n_feat};
     if (!x_scales) return launch_of<T>(d->x, d->x_sm, d->M, d->D, W, K, few, st, who);
     // (tiles that do not go round in one wait for their tokens' RoPE rows too
-    // often: 128 x 8192 x 10305 37.4 us against 33.8)
-    if (p || few_rows(X) || (d->M <= kFewRows && tiles_of(X, W, 64, 64) > device_cus()))
+    // often: 128 x 8192 x 10305 37.4 us against 33.8; in one of 96 x 64 25.8)
+    if (p || few_rows(X, W) ||
+        (d->M <= kFewRows && tiles_of(X, W, 64, 64) > device_cus() && !one_round_of_96(X, W, K)))
       return launch_few(X, W, K, few, st, who);
     if constexpr (sizeof(T) == 2)
       if (d->Dh % 8 == 0) return launch_many(X, W, K, FrontSink<T, false, 8>{*d, tab, len, n_feat}, st, who);

@@ -220,7 +220,7 @@ def test_linear_int8(M, K, N, dtype):
 
 
 @pytest.mark.parametrize("K", [1, 128, 129, 300, 384, 512, 520, 640, 896, 1000, 1152])
-@pytest.mark.parametrize("M,N", [(70, 500), (200, 1030), (128, 10305), (130, 9000), (250, 4100)])
+@pytest.mark.parametrize("M,N", [(70, 500), (200, 1030), (128, 10305), (130, 9000), (250, 4100), (190, 8100)])
 def test_shares_of_k(M, K, N):
     """Few and odd numbers of steps where several waves share K: some have one
     step more than others, or none."""
